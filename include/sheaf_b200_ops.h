@@ -183,9 +183,101 @@ SB_API int sb_op_get_batch(const void* data, int64_t n, const void* key, int32_t
  * (child i = threefry(key, [i, 1]), prng.rs:81-84, random_ops.rs:146-162). */
 SB_API int sb_op_random_split(const void* key, int32_t n, void* out, void* stream);
 
-/* Reads and clears the device error word that bounded waits inside the
- * kernels set (0 = no error, 1 = a barrier wait timed out). Synchronizes
- * the device. */
+/* ---- cached generation and scoring -------------------------------------
+ * The reference has no cache: its sampler runs the whole window for every
+ * token (examples/nanogpt/sample.shf:28-45), and its loss gives the mean over
+ * the rows alone (sheaf/lib/nn.shf:44-50). These serve callers that draw
+ * several answers to one prompt inside the context and learn from the answers'
+ * log probabilities. Index arguments (sequences, positions, page tables,
+ * lengths) are int32 device arrays; strides are in elements. */
+
+/* One layer's paged key / value cache: row r of head h of page p starts at
+ * element p * page_stride + r * row_stride + h * head_stride of `k` and `v`.
+ * `k`, `v` and the strides (in bytes) are multiples of 16 bytes; a head's
+ * head_dim values are contiguous. */
+typedef struct sb_kv_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, row_stride, head_stride;
+  int32_t n_pages, page_rows, n_heads, head_dim;
+  uint32_t elem; /* SB_ELEM_BF16 or SB_ELEM_F32 */
+} sb_kv_cache;
+
+#define SB_ROTARY_NONE 0
+#define SB_ROTARY_HALVES 1 /* value i turns with value i + rot_dim / 2 */
+#define SB_ROTARY_PAIRS 2  /* value 2 i turns with value 2 i + 1 */
+
+/* Appends n tokens' keys and values. qkv [n, (h_q + 2 * n_heads) * head_dim]
+ * (q | k | v, row stride ld) in the cache's element type; token i belongs to
+ * sequence seq[i] at position pos[i], whose own page table (row seq[i] of
+ * pages [n_seqs, max_pages]) starts at position `base`: it is written to page
+ * pages[seq][(pos - base) / page_rows], row (pos - base) % page_rows. The
+ * first rot_dim values of each query and key head are rotated by row pos of
+ * cos_table / sin_table (f32 [n_pos, rot_dim / 2]); the queries go to q_out
+ * [n, h_q * head_dim] (row stride ldq), which may be qkv itself with ldq = ld.
+ * seq[i] < 0 marks padding: nothing is appended, its q_out row is zero. A
+ * token whose sequence, position or page lies outside its table is treated
+ * likewise (a page outside the cache: its q_out row is still computed) and
+ * sb_op_device_error reports 2. With h_q = 0, qkv is k | v and q_out NULL.
+ * head_dim: 32, 64 or 128. */
+SB_API int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld, int32_t n, int32_t h_q, void* q_out,
+                           int64_t ldq, const void* seq, const void* pos, int32_t base, const void* pages,
+                           int32_t n_seqs, int32_t max_pages, int32_t rotary, int32_t rot_dim, const void* cos_table,
+                           const void* sin_table, int32_t n_pos, void* stream);
+
+/* Attention of b sequences that share their first prefix_len keys: sequence s
+ * has those (in pages prefix_pages[0 .. ceil(prefix_len / page_rows))), then
+ * lens[s] keys of its own (pages[s], row stride max_pages), the last tq of
+ * which belong to its tq query tokens. Query t of sequence s sees the keys up
+ * to its own, number prefix_len + lens[s] - tq + t:
+ *   out = softmax(scale * q k^T) v,  lse = log sum exp(scale * q k^T)
+ * q, out [b * tq, h_q * head_dim] (row strides ldq, ldo; query head h reads
+ * key head h / (h_q / n_heads)) in the cache's element type; lse f32
+ * [b * tq, h_q], or NULL. A query that sees no key (lens[s] < 0 marks an idle
+ * slot) gets a zero row and lse = -inf. prefix_len = 0 is plain attention
+ * over a paged cache, max_pages = 0 attention to the prefix alone. lens[s]
+ * beyond its table counts as the table's capacity and a page outside the
+ * cache as page 0; sb_op_device_error then reports 2. scale > 0. q, out and
+ * their row strides are multiples of 16 bytes. head_dim: 32, 64 or 128. */
+SB_API size_t sb_op_prefix_attention_workspace_size(const sb_kv_cache* cache, int32_t b, int32_t tq, int32_t h_q,
+                                                    int32_t prefix_len, int32_t max_pages);
+SB_API int sb_op_prefix_attention(const sb_kv_cache* cache, const void* q, int64_t ldq, void* out, int64_t ldo,
+                                  void* lse, int32_t b, int32_t tq, int32_t h_q, float scale, const void* prefix_pages,
+                                  int32_t prefix_len, const void* pages, int32_t max_pages, const void* lens,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scores rows of logits [rows, v] (row stride ld, any alignment) at a
+ * temperature > 0, with z = logits / temperature:
+ *   logp [rows]    = z[t] - lse for the row's given token t (f32 class id as
+ *                    in sb_op_cross_entropy: one that is not exactly an
+ *                    integer in [0, v) gives 0)
+ *   entropy [rows] = -sum_j p_j log p_j, p = softmax(z)
+ *   lse [rows]     = log sum_j exp z_j
+ *   top_ids, top_logp [rows, k] = the k likeliest tokens (i32), the larger
+ *                    logit first, equal ones by the lower index, and their
+ *                    log probabilities; 0 <= k <= min(v, 32)
+ * f32 outputs, each NULL when not wanted (targets are needed for logp alone).
+ * A logit of -inf has probability 0; a row of nothing else has lse = -inf and
+ * entropy 0. A row with a NaN or +inf has NaN statistics, and a NaN orders
+ * before every number. */
+#define SB_LOGPROBS_MAX_TOP 32
+SB_API int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v,
+                                const void* targets, float temperature, void* logp, void* entropy, void* lse,
+                                int32_t k, void* top_ids, void* top_logp, void* stream);
+/* Its VJP in logp and entropy, from the lse and entropy it gave:
+ *   dlogits_j = (dlogp (1[j = t] - p_j) - dentropy p_j (log p_j + entropy)) / temperature
+ * dlogits [rows, v] (row stride ldd) in the logits' type; it may be the
+ * logits' own memory with ldd = ld. dlogp, dentropy f32 [rows], either NULL
+ * for none (targets are needed with dlogp, entropy with dentropy). A row whose
+ * lse is -inf has a zero gradient. */
+SB_API int sb_op_token_logprobs_bwd(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v,
+                                    const void* targets, float temperature, const void* lse, const void* entropy,
+                                    const void* dlogp, const void* dentropy, void* dlogits, int64_t ldd,
+                                    void* stream);
+
+/* Reads and clears the device error word that kernels set (0 = no error,
+ * 1 = a barrier wait timed out, 2 = an index outside its table or cache).
+ * Synchronizes the device. */
 SB_API int sb_op_device_error(void);
 
 #ifdef __cplusplus

@@ -36,6 +36,13 @@ class SamplerConfig(C.Structure):
     _fields_ = [("n_new", C.c_int32), ("top_k", C.c_int32), ("temperature", C.c_float)]
 
 
+class KvCache(C.Structure):
+    """sb_kv_cache (include/sheaf_b200_ops.h): one layer's paged keys and values."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("n_pages", C.c_int32), ("page_rows", C.c_int32), ("n_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("elem", C.c_uint32)]
+
+
 class SessionStats(C.Structure):
     """sb_session_stats (include/sheaf_b200.h)."""
     _fields_ = [("calls", C.c_uint64), ("graph_captures", C.c_uint64), ("graph_replays", C.c_uint64),
@@ -78,6 +85,16 @@ SIGNATURES: dict[str, tuple] = {
                                    _P]),
     "sb_op_global_norm": (C.c_int, [C.c_uint32, C.c_int32, C.POINTER(C.c_int64), C.POINTER(_P), _P, _P, C.c_size_t,
                                     _P]),
+    "sb_op_kv_append": (C.c_int, [C.POINTER(KvCache), _P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P,
+                                  C.c_int32, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int32, _P]),
+    "sb_op_prefix_attention_workspace_size": (C.c_size_t, [C.POINTER(KvCache), C.c_int32, C.c_int32, C.c_int32,
+                                                           C.c_int32, C.c_int32]),
+    "sb_op_prefix_attention": (C.c_int, [C.POINTER(KvCache), _P, C.c_int64, _P, C.c_int64, _P, C.c_int32, C.c_int32,
+                                         C.c_int32, C.c_float, _P, C.c_int32, _P, C.c_int32, _P, _P, C.c_size_t, _P]),
+    "sb_op_token_logprobs": (C.c_int, [C.c_uint32, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_float, _P, _P, _P,
+                                       C.c_int32, _P, _P, _P]),
+    "sb_op_token_logprobs_bwd": (C.c_int, [C.c_uint32, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_float, _P, _P, _P,
+                                           _P, _P, C.c_int64, _P]),
     "sb_op_device_error": (C.c_int, []),
     # sheaf_b200.h
     "sb_status_is_ok": (C.c_bool, [_P]),

@@ -1,9 +1,11 @@
 // C-ABI wrappers of the kernel library (include/sheaf_b200_ops.h).
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "../../include/sheaf_b200_ops.h"
+#include "sb_cache.h"
 #include "sb_kernels.h"
 #include "sb_nn.h"
 
@@ -216,6 +218,174 @@ int sb_op_global_norm(uint32_t elem, int32_t n_leaves, const int64_t* counts, co
                             nullptr, nullptr, nullptr, nullptr, nullptr, 0.f, 0.f, 0.f, 0.f, 0.f,
                             static_cast<float*>(norm_out), workspace, workspace_bytes,
                             static_cast<cudaStream_t>(stream));
+}
+
+static bool fits(int64_t v) { return v > -(int64_t{1} << 40) && v < (int64_t{1} << 40); }
+
+// A usable cache description: strides that keep every 16-byte vector aligned
+// (rows of a head never overlap a neighbour's by less than head_dim).
+static int check_cache(const sb_kv_cache* c) {
+  if (!c || !float_elem(c->elem)) return SB_OPERR_ARGS;
+  if (c->n_heads <= 0 || c->page_rows <= 0 || c->n_pages < 0) return SB_OPERR_ARGS;
+  if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return SB_OPERR_ARGS;
+  if (c->n_pages > 0 && (!c->k || !c->v)) return SB_OPERR_ARGS;
+  const int64_t vec = c->elem == SB_ELEM_F32 ? 4 : 8;
+  if (!fits(c->page_stride) || !fits(c->row_stride) || !fits(c->head_stride)) return SB_OPERR_ARGS;
+  if (c->page_stride < 0 || c->row_stride < 0 || c->head_stride < 0) return SB_OPERR_ARGS;
+  if (c->page_stride % vec || c->row_stride % vec || c->head_stride % vec) return SB_OPERR_TMA;
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16) return SB_OPERR_TMA;
+  return 0;
+}
+
+int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld, int32_t n, int32_t h_q, void* q_out,
+                    int64_t ldq, const void* seq, const void* pos, int32_t base, const void* pages, int32_t n_seqs,
+                    int32_t max_pages, int32_t rotary, int32_t rot_dim, const void* cos_table, const void* sin_table,
+                    int32_t n_pos, void* stream) {
+  if (int rc = check_cache(cache)) return rc;
+  if (n < 0 || h_q < 0 || base < 0 || n_seqs < 0 || max_pages < 0) return SB_OPERR_ARGS;
+  if (rotary < SB_ROTARY_NONE || rotary > SB_ROTARY_PAIRS) return SB_OPERR_ARGS;
+  if (n == 0) return 0;
+  const int64_t heads = static_cast<int64_t>(h_q) + 2 * static_cast<int64_t>(cache->n_heads);
+  if (heads > (1 << 20)) return SB_OPERR_ARGS;
+  if (!qkv || !seq || !pos || !fits(ld) || ld < heads * cache->head_dim) return SB_OPERR_ARGS;
+  if ((n_seqs > 0 && max_pages > 0) && !pages) return SB_OPERR_ARGS;
+  if (h_q > 0 && (!q_out || !fits(ldq) || ldq < static_cast<int64_t>(h_q) * cache->head_dim)) return SB_OPERR_ARGS;
+  if (rotary != SB_ROTARY_NONE) {
+    if (rot_dim <= 0 || rot_dim % 2 || rot_dim > cache->head_dim || n_pos <= 0 || !cos_table || !sin_table)
+      return SB_OPERR_ARGS;
+  }
+  sb::AppendDesc d;
+  d.cache = *cache;
+  d.qkv = qkv;
+  d.ld = ld;
+  d.n = n;
+  d.h_q = h_q;
+  d.q_out = h_q > 0 ? q_out : nullptr;
+  d.ldq = ldq;
+  d.seq = static_cast<const int32_t*>(seq);
+  d.pos = static_cast<const int32_t*>(pos);
+  d.base = base;
+  d.pages = static_cast<const int32_t*>(pages);
+  d.n_seqs = n_seqs;
+  d.max_pages = max_pages;
+  d.rotary = rotary;
+  d.rot_dim = rot_dim;
+  d.cos = static_cast<const float*>(cos_table);
+  d.sin = static_cast<const float*>(sin_table);
+  d.n_pos = n_pos;
+  return sb::kv_append(d, static_cast<cudaStream_t>(stream), sb::device_error_word());
+}
+
+// The part of an attention call's arguments that its workspace depends on.
+static int fill_prefix_attn(sb::PrefixAttnDesc& d, const sb_kv_cache* cache, int32_t b, int32_t tq, int32_t h_q,
+                            int32_t prefix_len, int32_t max_pages) {
+  if (int rc = check_cache(cache)) return rc;
+  if (b < 0 || tq < 0 || h_q <= 0 || h_q % cache->n_heads || prefix_len < 0 || max_pages < 0) return SB_OPERR_ARGS;
+  // rows of queries and keys of a sequence are counted in 32 bits
+  if (static_cast<int64_t>(b) * tq * h_q > 0x7fffffff) return SB_OPERR_ARGS;
+  const int64_t own = static_cast<int64_t>(max_pages) * cache->page_rows;
+  if (own + prefix_len + tq > 0x7fff0000) return SB_OPERR_ARGS;
+  if (cache->n_pages == 0 && (prefix_len > 0 || max_pages > 0)) return SB_OPERR_ARGS;
+  d.cache = *cache;
+  d.b = b;
+  d.tq = tq;
+  d.h_q = h_q;
+  d.prefix_len = prefix_len;
+  d.max_pages = max_pages;
+  return 0;
+}
+
+size_t sb_op_prefix_attention_workspace_size(const sb_kv_cache* cache, int32_t b, int32_t tq, int32_t h_q,
+                                             int32_t prefix_len, int32_t max_pages) {
+  sb::PrefixAttnDesc d = {};
+  if (fill_prefix_attn(d, cache, b, tq, h_q, prefix_len, max_pages)) return 0;
+  return sb::prefix_attention_workspace_bytes(d);
+}
+
+int sb_op_prefix_attention(const sb_kv_cache* cache, const void* q, int64_t ldq, void* out, int64_t ldo, void* lse,
+                           int32_t b, int32_t tq, int32_t h_q, float scale, const void* prefix_pages,
+                           int32_t prefix_len, const void* pages, int32_t max_pages, const void* lens, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  sb::PrefixAttnDesc d = {};
+  if (int rc = fill_prefix_attn(d, cache, b, tq, h_q, prefix_len, max_pages)) return rc;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return SB_OPERR_ARGS;
+  if (b == 0 || tq == 0) return 0;
+  const int64_t width = static_cast<int64_t>(h_q) * cache->head_dim;
+  if (!q || !out || !lens || !fits(ldq) || !fits(ldo) || ldq < width || ldo < width) return SB_OPERR_ARGS;
+  if ((prefix_len > 0 && !prefix_pages) || (max_pages > 0 && !pages)) return SB_OPERR_ARGS;
+  const int64_t vec = cache->elem == SB_ELEM_F32 ? 4 : 8;
+  if (ldq % vec || ldo % vec || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
+    return SB_OPERR_TMA;
+  const size_t need = sb::prefix_attention_workspace_bytes(d);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return SB_OPERR_WORKSPACE;
+  d.q = q;
+  d.ldq = ldq;
+  d.out = out;
+  d.ldo = ldo;
+  d.lse = static_cast<float*>(lse);
+  d.scale = scale;
+  d.prefix_pages = static_cast<const int32_t*>(prefix_pages);
+  d.pages = static_cast<const int32_t*>(pages);
+  d.lens = static_cast<const int32_t*>(lens);
+  return sb::prefix_attention(d, workspace, workspace_bytes, static_cast<cudaStream_t>(stream),
+                              sb::device_error_word());
+}
+
+// Whether `p` is a pointer to whole values of the element type.
+static bool on_values(const void* p, uint32_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % (elem == SB_ELEM_F32 ? 4 : 2) == 0;
+}
+
+int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v, const void* targets,
+                         float temperature, void* logp, void* entropy, void* lse, int32_t k, void* top_ids,
+                         void* top_logp, void* stream) {
+  if (!float_elem(elem) || rows < 0 || v <= 0 || v > (1 << 30) || !fits(ld) || ld < v || k < 0 || k > SB_LOGPROBS_MAX_TOP || k > v)
+    return SB_OPERR_ARGS;
+  if (!(temperature > 0.f) || !std::isfinite(temperature)) return SB_OPERR_ARGS;
+  if (rows == 0) return 0;
+  if (!logits || !on_values(logits, elem) || (logp && !targets)) return SB_OPERR_ARGS;
+  sb::LogprobsDesc d;
+  d.f32 = elem == SB_ELEM_F32;
+  d.x = logits;
+  d.ld = ld;
+  d.rows = rows;
+  d.v = v;
+  d.targets = static_cast<const float*>(targets);
+  d.temperature = temperature;
+  d.logp = static_cast<float*>(logp);
+  d.entropy = static_cast<float*>(entropy);
+  d.lse = static_cast<float*>(lse);
+  d.k = top_ids || top_logp ? k : 0;
+  d.top_ids = static_cast<int32_t*>(top_ids);
+  d.top_logp = static_cast<float*>(top_logp);
+  return sb::token_logprobs(d, static_cast<cudaStream_t>(stream));
+}
+
+int sb_op_token_logprobs_bwd(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v,
+                             const void* targets, float temperature, const void* lse, const void* entropy,
+                             const void* dlogp, const void* dentropy, void* dlogits, int64_t ldd, void* stream) {
+  if (!float_elem(elem) || rows < 0 || v <= 0 || v > (1 << 30) || !fits(ld) || !fits(ldd) || ld < v || ldd < v) return SB_OPERR_ARGS;
+  if (!(temperature > 0.f) || !std::isfinite(temperature)) return SB_OPERR_ARGS;
+  if (rows == 0) return 0;
+  if (!logits || !dlogits || !lse || !on_values(logits, elem) || !on_values(dlogits, elem)) return SB_OPERR_ARGS;
+  if ((dlogp && !targets) || (dentropy && !entropy)) return SB_OPERR_ARGS;
+  if (dlogits == logits && ldd != ld) return SB_OPERR_ARGS;
+  sb::LogprobsBwdDesc d;
+  d.f32 = elem == SB_ELEM_F32;
+  d.x = logits;
+  d.ld = ld;
+  d.rows = rows;
+  d.v = v;
+  d.targets = static_cast<const float*>(targets);
+  d.temperature = temperature;
+  d.lse = static_cast<const float*>(lse);
+  d.entropy = static_cast<const float*>(entropy);
+  d.dlogp = static_cast<const float*>(dlogp);
+  d.dentropy = static_cast<const float*>(dentropy);
+  d.dx = dlogits;
+  d.ldd = ldd;
+  return sb::token_logprobs_bwd(d, static_cast<cudaStream_t>(stream));
 }
 
 int sb_op_device_error(void) {

@@ -1,0 +1,337 @@
+// Attention over a paged key / value cache whose sequences share a prefix:
+// dispatch, the CUDA-core kernel (float32), and the join of partial results.
+#include <algorithm>
+
+#include "prefix_attention.cuh"
+#include "sb_kernels.h"
+#define SB_PDL_FAMILY 2
+#include "sb_launch.cuh"
+
+namespace sb {
+
+int num_sms_cached();
+
+namespace {
+
+constexpr int kRows = 16;  // rows of a block: 4 warps of 4
+constexpr int kKeys = 32;  // keys of a tile: one a lane
+constexpr int kThreads = 128;
+
+template <int HD>
+struct SimtShared {
+  float q[kRows][HD];
+  float k[2][kKeys][HD + 4];  // padded: the lanes of a warp read a row each
+  float v[2][kKeys][HD];
+  float p[kThreads / 32][kKeys][4];
+};
+
+// Scores, softmax and output of 16 rows against a range of keys, all in
+// float32. A warp owns 4 rows: a lane computes the scores of its key with
+// them, then the output columns lane * HD / 32 .. over the tile's keys.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SimtShared<HD>& sh = *reinterpret_cast<SimtShared<HD>*>(smem_raw);
+  constexpr int C = HD / 32;  // output columns of a lane
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  pdl_wait();
+  const PaItem w = item_at(a, blockIdx.x, kRows, kKeys);
+  const int* table = table_of(a, w);
+  const bool prefix = w.seq < 0;
+
+  PaRow row[4];
+  int seen[4], most = 0, least = 0x7fffffff;  // keys that a row sees
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = w.row0 + warp * 4 + r;
+    seen[r] = 0;
+    if (i < w.rows) {
+      row[r] = row_of(a, w, i);
+      seen[r] = visible(a, prefix, row[r]);
+      least = min(least, seen[r]);
+    }
+    most = max(most, seen[r]);
+  }
+  const int k1 = min(w.k1, __syncthreads_or(most > w.k0) ? w.k1 : w.k0);
+  const int warp_k1 = min(k1, most);
+
+  for (int i = tid; i < kRows * HD; i += kThreads) {
+    const int r = w.row0 + i / HD;
+    float q = 0.f;
+    if (r < w.rows) {
+      const PaRow x = row_of(a, w, r);
+      q = static_cast<float>(static_cast<const T*>(a.q)[x.token * a.ldq + static_cast<long>(x.h) * HD + i % HD]);
+    }
+    sh.q[i / HD][i % HD] = q;
+  }
+
+  const auto load = [&](int stage, int j0) {
+    constexpr int V = 16 / sizeof(T), CH = HD / V;  // vectors of a row
+    for (int i = tid; i < kKeys * CH; i += kThreads) {
+      const int j = i / CH, c = i % CH * V;
+      const bool in = j0 + j < k1;
+      const long at = in ? key_offset(a, table, j0 + j) + w.head * a.head_stride + c : 0;
+      const T* k = static_cast<const T*>(a.k) + at;
+      const T* v = static_cast<const T*>(a.v) + at;
+      if constexpr (sizeof(T) == 4) {
+        cp_async16(smem_u32(&sh.k[stage][j][c]), k, in);
+        cp_async16(smem_u32(&sh.v[stage][j][c]), v, in);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sh.k[stage][j][c + e] = in ? static_cast<float>(k[e]) : 0.f;
+          sh.v[stage][j][c + e] = in ? static_cast<float>(v[e]) : 0.f;
+        }
+      }
+    }
+    cp_async_commit();
+  };
+
+  float m[4], l[4], o[4][C];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[r][c] = 0.f;
+  }
+  if (w.k0 < k1) load(0, w.k0);
+  int stage = 0;
+  for (int j0 = w.k0; j0 < k1; j0 += kKeys, stage ^= 1) {
+    if (j0 + kKeys < k1) {
+      load(stage ^ 1, j0 + kKeys);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    if (j0 < warp_k1) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+      for (int c = 0; c < HD; c += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(&sh.k[stage][lane][c]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 q = *reinterpret_cast<const float4*>(&sh.q[warp * 4 + r][c]);
+          s[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[r]))));
+        }
+      }
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[r] = j0 + lane < seen[r] ? s[r] * a.scale : -INFINITY;
+        float t = s[r];
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+        const float mn = fmaxf(m[r], t);
+        // a row that has seen no key keeps m = -inf, l = 0
+        const float f = mn == -INFINITY ? 1.f : expf(m[r] - mn);
+        p[r] = mn == -INFINITY ? 0.f : expf(s[r] - mn);
+        l[r] = l[r] * f + p[r];
+        m[r] = mn;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[r][c] *= f;
+      }
+      *reinterpret_cast<float4*>(&sh.p[warp][lane][0]) = make_float4(p[0], p[1], p[2], p[3]);
+      __syncwarp();
+      if (j0 + kKeys <= least) {
+#pragma unroll 8
+        for (int j = 0; j < kKeys; ++j) {
+          const float4 q = *reinterpret_cast<const float4*>(&sh.p[warp][j][0]);
+          float v[C];
+#pragma unroll
+          for (int c = 0; c < C; ++c) v[c] = sh.v[stage][j][lane * C + c];
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            o[0][c] = fmaf(q.x, v[c], o[0][c]);
+            o[1][c] = fmaf(q.y, v[c], o[1][c]);
+            o[2][c] = fmaf(q.z, v[c], o[2][c]);
+            o[3][c] = fmaf(q.w, v[c], o[3][c]);
+          }
+        }
+      } else {
+        // some row stops inside the tile: a key that it does not see must
+        // not reach it, whatever its values hold (0 * NaN)
+        const int n = min(kKeys, warp_k1 - j0);
+        for (int j = 0; j < n; ++j) {
+          const float4 q = *reinterpret_cast<const float4*>(&sh.p[warp][j][0]);
+          const float pr[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const float v = sh.v[stage][j][lane * C + c];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (j0 + j < seen[r]) o[r][c] = fmaf(pr[r], v, o[r][c]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (w.row0 + warp * 4 + r >= w.rows) continue;
+    float sum = l[r];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const long at = row[r].token * a.hq + row[r].h;
+    if (a.parts == 1) {
+      const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      T* out = static_cast<T*>(a.out) + row[r].token * a.ldo + static_cast<long>(row[r].h) * HD + lane * C;
+#pragma unroll
+      for (int c = 0; c < C; ++c) out[c] = static_cast<T>(o[r][c] * f);
+      if (a.lse && lane == 0) a.lse[at] = m[r] + logf(sum);
+    } else {
+      const long slot = static_cast<long>(w.part) * a.b * a.tq * a.hq + at;
+      if (lane == 0) a.part_ml[slot] = make_float2(m[r], sum);
+      if (sum != 0.f)
+#pragma unroll
+        for (int c = 0; c < C; ++c) a.part_o[slot * HD + lane * C + c] = o[r][c];
+    }
+  }
+}
+
+// A warp per row joins its partial results; a part that saw no key (l = 0)
+// left no output and is not read.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
+  constexpr int C = HD / 32;
+  pdl_wait();
+  const long rows = static_cast<long>(a.b) * a.tq * a.hq;
+  const long at = static_cast<long>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (at >= rows) return;
+  float m = -INFINITY;
+  for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, a.part_ml[p * rows + at].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  float l = 0.f, o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = 0.f;
+  for (int p = 0; p < a.parts; ++p) {
+    const float2 ml = a.part_ml[p * rows + at];
+    if (ml.y == 0.f) continue;
+    const float f = expf(ml.x - m);
+    l = fmaf(ml.y, f, l);
+    const float* src = a.part_o + (p * rows + at) * HD + lane * C;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = fmaf(src[c], f, o[c]);
+  }
+  const long token = at / a.hq;
+  const int h = static_cast<int>(at - token * a.hq);
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* out = static_cast<T*>(a.out) + token * a.ldo + static_cast<long>(h) * HD + lane * C;
+#pragma unroll
+  for (int c = 0; c < C; ++c) out[c] = static_cast<T>(o[c] * f);
+  if (a.lse && lane == 0) a.lse[at] = m + logf(l);
+}
+
+// How the keys of both segments are cut, and the launch that follows.
+struct Plan {
+  int prefix_splits = 0, own_splits = 0, prefix_tiles = 0, own_tiles = 0;
+  int parts() const { return prefix_splits + own_splits; }
+};
+
+long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+Plan plan_of(const PrefixAttnDesc& d) {
+  Plan p;
+  const long G = d.h_q / d.cache.n_heads, hkv = d.cache.n_heads;
+  const long prefix_keys = ceil_div(d.prefix_len, kKeys);
+  const long own_keys = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, kKeys);
+  p.prefix_tiles = static_cast<int>(ceil_div(static_cast<long>(d.b) * d.tq * G, kRows));
+  p.own_tiles = static_cast<int>(ceil_div(d.tq * G, kRows));
+  const long prefix_blocks = hkv * p.prefix_tiles, own_blocks = d.b * hkv * p.own_tiles;
+  // key tiles a block takes: at least 8, and enough that the blocks come out
+  // near two for each place on the GPU
+  const long total = prefix_blocks * prefix_keys + own_blocks * own_keys;
+  const long quota = std::max(8L, total / (4L * num_sms_cached()));
+  p.prefix_splits = static_cast<int>(std::min(64L, ceil_div(prefix_keys, quota)));
+  p.own_splits = static_cast<int>(std::min(64L, ceil_div(own_keys, quota)));
+  if (p.parts() == 0) p.own_splits = 1;  // no keys at all: one empty part
+  return p;
+}
+
+template <typename T, int HD>
+int run(const PaArgs& a, long items, cudaStream_t s) {
+  constexpr size_t smem = sizeof(SimtShared<HD>);
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(attn_simt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+      return SB_OPERR_LAUNCH;
+    attr = true;
+  }
+  launch_pdl(attn_simt_kernel<T, HD>, dim3(static_cast<unsigned>(items)), dim3(kThreads), smem, s, a);
+  if (a.parts > 1) {
+    const long rows = static_cast<long>(a.b) * a.tq * a.hq;
+    launch_pdl(attn_join_kernel<T, HD>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, a);
+  }
+  return cudaPeekAtLastError() == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
+}
+
+template <typename T>
+int run_t(const PaArgs& a, int hd, long items, cudaStream_t s) {
+  if (hd == 32) return run<T, 32>(a, items, s);
+  if (hd == 64) return run<T, 64>(a, items, s);
+  return run<T, 128>(a, items, s);
+}
+
+size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
+
+}  // namespace
+
+size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {
+  const int parts = plan_of(d).parts();
+  if (parts <= 1) return 0;
+  const size_t rows = static_cast<size_t>(d.b) * d.tq * d.h_q;
+  return align16(parts * rows * sizeof(float2)) + parts * rows * d.cache.head_dim * sizeof(float);
+}
+
+int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, int* err) {
+  const Plan p = plan_of(d);
+  PaArgs a = {};
+  a.k = d.cache.k;
+  a.v = d.cache.v;
+  a.page_stride = d.cache.page_stride;
+  a.row_stride = d.cache.row_stride;
+  a.head_stride = d.cache.head_stride;
+  a.n_pages = d.cache.n_pages;
+  a.hkv = d.cache.n_heads;
+  a.page_rows = FastDiv::of(d.cache.page_rows);
+  a.q = d.q;
+  a.ldq = d.ldq;
+  a.out = d.out;
+  a.ldo = d.ldo;
+  a.lse = d.lse;
+  a.b = d.b;
+  a.tq = d.tq;
+  a.hq = d.h_q;
+  a.group = FastDiv::of(d.h_q / d.cache.n_heads);
+  a.seq_rows = FastDiv::of(d.tq * (d.h_q / d.cache.n_heads));
+  a.scale = d.scale;
+  a.prefix_pages = d.prefix_pages;
+  a.prefix_len = d.prefix_len;
+  a.pages = d.pages;
+  a.max_pages = d.max_pages;
+  a.capacity = d.max_pages * d.cache.page_rows;
+  a.lens = d.lens;
+  a.parts = p.parts();
+  a.prefix_splits = p.prefix_splits;
+  a.own_splits = p.own_splits;
+  a.prefix_tiles = p.prefix_tiles;
+  a.own_tiles = p.own_tiles;
+  const size_t rows = static_cast<size_t>(d.b) * d.tq * d.h_q;
+  a.part_ml = static_cast<float2*>(ws);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align16(a.parts * rows * sizeof(float2)));
+  a.err = err;
+  const long prefix_items = static_cast<long>(a.hkv) * p.prefix_tiles * p.prefix_splits;
+  const long items = prefix_items + static_cast<long>(d.b) * a.hkv * p.own_tiles * p.own_splits;
+  if (items > 0x7fffffffL) return SB_OPERR_ARGS;
+  a.prefix_items = static_cast<int>(prefix_items);
+  return d.cache.elem == SB_ELEM_F32 ? run_t<float>(a, d.cache.head_dim, items, s)
+                                     : run_t<__nv_bfloat16>(a, d.cache.head_dim, items, s);
+}
+
+}  // namespace sb
