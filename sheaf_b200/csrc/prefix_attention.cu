@@ -28,14 +28,11 @@ struct SimtShared {
 // Scores, softmax and output of 16 rows against a range of keys, all in
 // float32. A warp owns 4 rows: a lane computes the scores of its key with
 // them, then the output columns lane * HD / 32 .. over the tile's keys.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  SimtShared<HD>& sh = *reinterpret_cast<SimtShared<HD>*>(smem_raw);
+template <int HD>
+__device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& sh) {
+  using T = float;
   constexpr int C = HD / 32;  // output columns of a lane
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  pdl_wait();
-  const PaItem w = item_at(a, blockIdx.x, kRows, kKeys);
   const int* table = table_of(a, w);
   const bool prefix = w.seq < 0;
 
@@ -52,7 +49,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
     }
     most = max(most, seen[r]);
   }
-  const int k1 = min(w.k1, __syncthreads_or(most > w.k0) ? w.k1 : w.k0);
+  const int k1 = __syncthreads_or(most > w.k0) ? w.k1 : w.k0;  // shared memory is free, too
   const int warp_k1 = min(k1, most);
 
   for (int i = tid; i < kRows * HD; i += kThreads) {
@@ -73,16 +70,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
       const long at = in ? key_offset(a, table, j0 + j) + w.head * a.head_stride + c : 0;
       const T* k = static_cast<const T*>(a.k) + at;
       const T* v = static_cast<const T*>(a.v) + at;
-      if constexpr (sizeof(T) == 4) {
-        cp_async16(smem_u32(&sh.k[stage][j][c]), k, in);
-        cp_async16(smem_u32(&sh.v[stage][j][c]), v, in);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          sh.k[stage][j][c + e] = in ? static_cast<float>(k[e]) : 0.f;
-          sh.v[stage][j][c + e] = in ? static_cast<float>(v[e]) : 0.f;
-        }
-      }
+      cp_async16(smem_u32(&sh.k[stage][j][c]), k, in);
+      cp_async16(smem_u32(&sh.v[stage][j][c]), v, in);
     }
     cp_async_commit();
   };
@@ -176,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     const long at = row[r].token * a.hq + row[r].h;
-    if (a.parts == 1) {
+    if (a.direct) {
       const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
       T* out = static_cast<T*>(a.out) + row[r].token * a.ldo + static_cast<long>(row[r].h) * HD + lane * C;
 #pragma unroll
@@ -192,6 +181,23 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
   }
 }
 
+// Blocks [0, prefix blocks) take runs of the prefix, the others own pieces.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SimtShared<HD>& sh = *reinterpret_cast<SimtShared<HD>*>(smem_raw);
+  pdl_wait();
+  pdl_trigger();
+  const int cta = blockIdx.x;
+  if (cta < a.prefix.ctas) {
+    PaRun run(a.prefix, a.hkv, cta);
+    PaPiece w;
+    while (run.next(a, cta, w)) attend_piece<HD>(a, w, sh);
+  } else {
+    attend_piece<HD>(a, own_piece(a, cta - a.prefix.ctas), sh);
+  }
+}
+
 // A warp per row joins its partial results; a part that saw no key (l = 0)
 // left no output and is not read.
 template <typename T, int HD>
@@ -202,24 +208,36 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   const long at = static_cast<long>(blockIdx.x) * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (at >= rows) return;
+  const long token = at / a.hq;
+  const int h = static_cast<int>(at - token * a.hq);
+  int n_prefix = 0;
+  if (a.prefix.ctas > 0) {
+    const int head = a.group(h);
+    const long row = token * a.group.d + (h - head * static_cast<int>(a.group.d));
+    n_prefix = a.prefix.parts_of(head * a.prefix.row_tiles + static_cast<int>(row / a.prefix.tile_rows));
+  }
+  const int parts = n_prefix + a.own.splits;
+  const auto slot = [&](int p) { return (p < n_prefix ? p : a.prefix.parts + p - n_prefix) * rows + at; };
   float m = -INFINITY;
-  for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, a.part_ml[p * rows + at].x);
+  for (int p = lane; p < parts; p += 32) {
+    const float2 ml = a.part_ml[slot(p)];
+    if (ml.y != 0.f) m = fmaxf(m, ml.x);
+  }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   float l = 0.f, o[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = 0.f;
-  for (int p = 0; p < a.parts; ++p) {
-    const float2 ml = a.part_ml[p * rows + at];
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = a.part_ml[slot(p)];
     if (ml.y == 0.f) continue;
     const float f = expf(ml.x - m);
     l = fmaf(ml.y, f, l);
-    const float* src = a.part_o + (p * rows + at) * HD + lane * C;
+    const float* src = a.part_o + slot(p) * HD + lane * C;
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] = fmaf(src[c], f, o[c]);
   }
-  const long token = at / a.hq;
-  const int h = static_cast<int>(at - token * a.hq);
   const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* out = static_cast<T*>(a.out) + token * a.ldo + static_cast<long>(h) * HD + lane * C;
 #pragma unroll
@@ -227,70 +245,87 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   if (a.lse && lane == 0) a.lse[at] = m + logf(l);
 }
 
-// How the keys of both segments are cut, and the launch that follows.
+// How the keys of both segments are cut.
 struct Plan {
-  int prefix_splits = 0, own_splits = 0, prefix_tiles = 0, own_tiles = 0;
-  int parts() const { return prefix_splits + own_splits; }
+  PaPrefix prefix = {};
+  PaOwn own = {};
+  int own_ctas = 0;
+  long parts() const { return prefix.parts + own.splits; }
 };
 
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-Plan plan_of(const PrefixAttnDesc& d) {
-  Plan p;
+bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long G = d.h_q / d.cache.n_heads, hkv = d.cache.n_heads;
-  const long prefix_keys = ceil_div(d.prefix_len, kKeys);
-  const long own_keys = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, kKeys);
-  p.prefix_tiles = static_cast<int>(ceil_div(static_cast<long>(d.b) * d.tq * G, kRows));
-  p.own_tiles = static_cast<int>(ceil_div(d.tq * G, kRows));
-  const long prefix_blocks = hkv * p.prefix_tiles, own_blocks = d.b * hkv * p.own_tiles;
-  // key tiles a block takes: at least 8, and enough that the blocks come out
-  // near two for each place on the GPU
-  const long total = prefix_blocks * prefix_keys + own_blocks * own_keys;
-  const long quota = std::max(8L, total / (4L * num_sms_cached()));
-  p.prefix_splits = static_cast<int>(std::min(64L, ceil_div(prefix_keys, quota)));
-  p.own_splits = static_cast<int>(std::min(64L, ceil_div(own_keys, quota)));
-  if (p.parts() == 0) p.own_splits = 1;  // no keys at all: one empty part
-  return p;
+  const bool f32 = d.cache.elem == SB_ELEM_F32;
+  const long prefix_rows = static_cast<long>(d.b) * d.tq * G, own_rows = d.tq * G;
+  const auto tile_rows = [&](long rows) { return f32 || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); };
+  const int tile_keys = f32 ? kKeys : 64;
+  p.prefix.tile_rows = tile_rows(prefix_rows);
+  p.own.tile_rows = tile_rows(own_rows);
+  p.prefix.tile_keys = p.own.tile_keys = tile_keys;
+  p.prefix.row_tiles = static_cast<int>(ceil_div(prefix_rows, p.prefix.tile_rows));
+  p.own.row_tiles = static_cast<int>(ceil_div(own_rows, p.own.tile_rows));
+  p.prefix.tiles = static_cast<int>(ceil_div(d.prefix_len, tile_keys));
+  const long own_tiles = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, tile_keys);
+  const long prefix_work = hkv * p.prefix.row_tiles * p.prefix.tiles;
+  const long own_items = d.b * hkv * p.own.row_tiles;
+  // key tiles that a block takes: at least 2, and enough that all blocks fit
+  // two to an SM
+  const long quota = std::max(2L, ceil_div(prefix_work + own_items * own_tiles, 2L * num_sms_cached()));
+  if (quota > 0x7fffffffL) return false;
+  p.prefix.per_cta = static_cast<int>(quota);
+  p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, quota));
+  p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / quota + 2) : 0;
+  if (p.prefix.tiles > 0 && quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
+  p.own.splits = static_cast<int>(std::min(64L, ceil_div(own_tiles, quota)));
+  if (p.parts() == 0) p.own.splits = 1;  // no keys at all: one empty part
+  const long own_ctas = own_items * p.own.splits;
+  if (own_ctas + p.prefix.ctas > 0x7fffffffL) return false;
+  p.own_ctas = static_cast<int>(own_ctas);
+  return true;
 }
 
-template <typename T, int HD>
-int run(const PaArgs& a, long items, cudaStream_t s) {
+template <int HD>
+int simt(const PaArgs& a, int own_ctas, cudaStream_t s) {
   constexpr size_t smem = sizeof(SimtShared<HD>);
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(attn_simt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(attn_simt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem)) != cudaSuccess)
       return SB_OPERR_LAUNCH;
     attr = true;
   }
-  launch_pdl(attn_simt_kernel<T, HD>, dim3(static_cast<unsigned>(items)), dim3(kThreads), smem, s, a);
-  if (a.parts > 1) {
-    const long rows = static_cast<long>(a.b) * a.tq * a.hq;
-    launch_pdl(attn_join_kernel<T, HD>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, a);
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
+  return launch_pdl(attn_simt_kernel<HD>, dim3(static_cast<unsigned>(a.prefix.ctas) + own_ctas), dim3(kThreads), smem,
+                    s, a) == cudaSuccess
+             ? 0
+             : SB_OPERR_LAUNCH;
 }
 
 template <typename T>
-int run_t(const PaArgs& a, int hd, long items, cudaStream_t s) {
-  if (hd == 32) return run<T, 32>(a, items, s);
-  if (hd == 64) return run<T, 64>(a, items, s);
-  return run<T, 128>(a, items, s);
+int join(const PaArgs& a, int hd, cudaStream_t s) {
+  const long rows = static_cast<long>(a.b) * a.tq * a.hq;
+  const dim3 grid(static_cast<unsigned>((rows + 7) / 8));
+  const auto k = hd == 32 ? attn_join_kernel<T, 32> : (hd == 64 ? attn_join_kernel<T, 64> : attn_join_kernel<T, 128>);
+  return launch_pdl(k, grid, dim3(256), 0, s, a) == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
 }
 
 size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
 
 }  // namespace
 
+int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
+
 size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {
-  const int parts = plan_of(d).parts();
-  if (parts <= 1) return 0;
+  Plan p;
+  if (d.b == 0 || d.tq == 0 || !plan_of(d, p) || p.parts() <= 1) return 0;
   const size_t rows = static_cast<size_t>(d.b) * d.tq * d.h_q;
-  return align16(parts * rows * sizeof(float2)) + parts * rows * d.cache.head_dim * sizeof(float);
+  return align16(p.parts() * rows * sizeof(float2)) + p.parts() * rows * d.cache.head_dim * sizeof(float);
 }
 
 int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, int* err) {
-  const Plan p = plan_of(d);
+  Plan p;
+  if (!plan_of(d, p)) return SB_OPERR_ARGS;
   PaArgs a = {};
   a.k = d.cache.k;
   a.v = d.cache.v;
@@ -317,21 +352,22 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   a.max_pages = d.max_pages;
   a.capacity = d.max_pages * d.cache.page_rows;
   a.lens = d.lens;
-  a.parts = p.parts();
-  a.prefix_splits = p.prefix_splits;
-  a.own_splits = p.own_splits;
-  a.prefix_tiles = p.prefix_tiles;
-  a.own_tiles = p.own_tiles;
+  a.prefix = p.prefix;
+  a.own = p.own;
+  a.direct = p.parts() == 1;
   const size_t rows = static_cast<size_t>(d.b) * d.tq * d.h_q;
   a.part_ml = static_cast<float2*>(ws);
-  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align16(a.parts * rows * sizeof(float2)));
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align16(p.parts() * rows * sizeof(float2)));
   a.err = err;
-  const long prefix_items = static_cast<long>(a.hkv) * p.prefix_tiles * p.prefix_splits;
-  const long items = prefix_items + static_cast<long>(d.b) * a.hkv * p.own_tiles * p.own_splits;
-  if (items > 0x7fffffffL) return SB_OPERR_ARGS;
-  a.prefix_items = static_cast<int>(prefix_items);
-  return d.cache.elem == SB_ELEM_F32 ? run_t<float>(a, d.cache.head_dim, items, s)
-                                     : run_t<__nv_bfloat16>(a, d.cache.head_dim, items, s);
+  const int hd = d.cache.head_dim;
+  const bool f32 = d.cache.elem == SB_ELEM_F32;
+  int rc;
+  if (!f32)
+    rc = attn_mma(a, hd, a.prefix.ctas, p.own_ctas, s);
+  else
+    rc = hd == 32 ? simt<32>(a, p.own_ctas, s) : (hd == 64 ? simt<64>(a, p.own_ctas, s) : simt<128>(a, p.own_ctas, s));
+  if (rc || a.direct) return rc;
+  return f32 ? join<float>(a, hd, s) : join<__nv_bfloat16>(a, hd, s);
 }
 
 }  // namespace sb

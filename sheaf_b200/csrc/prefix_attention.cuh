@@ -39,6 +39,27 @@ struct FastDiv {
   }
 };
 
+// How the prefix's work is cut: items (key head, tile of rows) of `tiles` key
+// tiles each, one after the other, in runs of `per_cta` key tiles a block,
+// whatever items a run touches. Item i leaves its part n = block - first(i).
+struct PaPrefix {
+  int row_tiles;  // of a key head
+  int tile_rows, tile_keys;
+  int tiles, per_cta, ctas;
+  int parts;      // most parts an item has
+  __host__ __device__ __forceinline__ int first(int item) const {
+    return static_cast<int>(static_cast<long>(item) * tiles / per_cta);
+  }
+  __host__ __device__ __forceinline__ int parts_of(int item) const {
+    return static_cast<int>((static_cast<long>(item + 1) * tiles - 1) / per_cta) - first(item) + 1;
+  }
+};
+// The sequences' own keys: items (sequence, key head, tile of rows), each cut
+// evenly into `splits`, a block each.
+struct PaOwn {
+  int row_tiles, tile_rows, tile_keys, splits;
+};
+
 struct PaArgs {
   const void* k;
   const void* v;
@@ -51,33 +72,33 @@ struct PaArgs {
   long ldo;
   float* lse;
   int b, tq, hq;
-  FastDiv group;      // G = hq / hkv
-  FastDiv seq_rows;   // tq * G
+  FastDiv group;     // G = hq / hkv
+  FastDiv seq_rows;  // tq * G
   float scale;
   const int* prefix_pages;
   int prefix_len;
   const int* pages;
   int max_pages;
-  int capacity;       // max_pages * page_rows
+  int capacity;      // max_pages * page_rows
   const int* lens;
-  // partial results: o [parts][b * tq * hq][hd], ml [parts][b * tq * hq]
+  PaPrefix prefix;
+  PaOwn own;
+  // partial results: o [parts][b * tq * hq][hd], ml [parts][b * tq * hq];
+  // parts: the prefix's, then the own splits'
   float* part_o;
   float2* part_ml;
-  int parts;          // prefix splits, then own splits
-  int prefix_splits, own_splits;
-  int prefix_tiles, own_tiles;  // row tiles of a key head / of a (sequence, key head)
-  int prefix_items;   // hkv * prefix_tiles * prefix_splits
+  bool direct;       // there is one part: results go straight to out, lse
   int* err;
 };
 
 // A block of rows against a range of one segment's keys.
-struct PaItem {
-  int seq;        // -1: the prefix
-  int head;       // key head
-  int row0;       // first of the tile's rows among the segment's
-  int rows;       // the segment's rows
-  int part;       // where its partial results go
-  int k0, k1;     // keys
+struct PaPiece {
+  int seq;     // -1: the prefix
+  int head;    // key head
+  int row0;    // first of the tile's rows among the segment's
+  int rows;    // the segment's rows
+  int part;    // where its partial results go
+  int k0, k1;  // keys
 };
 
 __device__ __forceinline__ int seq_len(const PaArgs& a, int s) {
@@ -94,7 +115,7 @@ struct PaRow {
   int s, t, h;
   long token;  // s * tq + t
 };
-__device__ __forceinline__ PaRow row_of(const PaArgs& a, const PaItem& w, int i) {
+__device__ __forceinline__ PaRow row_of(const PaArgs& a, const PaPiece& w, int i) {
   PaRow r;
   int in_seq = i;
   r.s = w.seq;
@@ -108,7 +129,7 @@ __device__ __forceinline__ PaRow row_of(const PaArgs& a, const PaItem& w, int i)
   return r;
 }
 
-// How many of the segment's keys row r sees (a prefix of them).
+// How many of the segment's keys row r sees (the first ones).
 __device__ __forceinline__ int visible(const PaArgs& a, bool prefix, const PaRow& r) {
   const int n = seq_len(a, r.s);
   if (n < 0) return 0;
@@ -117,39 +138,52 @@ __device__ __forceinline__ int visible(const PaArgs& a, bool prefix, const PaRow
   return max(min(a.prefix_len + own, a.prefix_len), 0);
 }
 
-// Item `i` of the launch: the prefix's items, row tiles fastest (blocks that
-// run together share keys), then the sequences' own.
-__device__ __forceinline__ PaItem item_at(const PaArgs& a, int i, int tile_rows, int tile_keys) {
-  PaItem w;
-  int len, splits, split;
-  if (i < a.prefix_items) {
-    const int tile = i % a.prefix_tiles;
-    i /= a.prefix_tiles;
-    w.seq = -1;
-    w.head = i % a.hkv;
-    split = i / a.hkv;
-    w.row0 = tile * tile_rows;
-    w.rows = a.b * a.seq_rows.d;
-    w.part = split;
-    len = a.prefix_len;
-    splits = a.prefix_splits;
-  } else {
-    i -= a.prefix_items;
-    const int tile = i % a.own_tiles;
-    i /= a.own_tiles;
-    w.head = i % a.hkv;
-    i /= a.hkv;
-    w.seq = i / a.own_splits;
-    split = i - w.seq * a.own_splits;
-    w.row0 = tile * tile_rows;
-    w.rows = a.seq_rows.d;
-    w.part = a.prefix_splits + split;
-    len = max(seq_len(a, w.seq), 0);
-    splits = a.own_splits;
+// The pieces of a block that takes a run of the prefix's key tiles.
+struct PaRun {
+  long at, end;
+  __device__ __forceinline__ PaRun(const PaPrefix& p, int hkv, int cta) {
+    at = static_cast<long>(cta) * p.per_cta;
+    end = min(at + p.per_cta, static_cast<long>(hkv) * p.row_tiles * p.tiles);
   }
-  const int tiles = (len + tile_keys - 1) / tile_keys;
-  w.k0 = static_cast<int>(static_cast<long>(tiles) * split / splits) * tile_keys;
-  w.k1 = min(static_cast<int>(static_cast<long>(tiles) * (split + 1) / splits) * tile_keys, len);
+  __device__ __forceinline__ bool next(const PaArgs& a, int cta, PaPiece& w) {
+    if (at >= end) return false;
+    const PaPrefix& p = a.prefix;
+    const int item = static_cast<int>(at / p.tiles);
+    const int t0 = static_cast<int>(at - static_cast<long>(item) * p.tiles);
+    const int t1 = static_cast<int>(min(end - static_cast<long>(item) * p.tiles, static_cast<long>(p.tiles)));
+    w.seq = -1;
+    w.head = item / p.row_tiles;
+    w.row0 = (item - w.head * p.row_tiles) * p.tile_rows;
+    w.rows = a.b * a.seq_rows.d;
+    w.part = cta - p.first(item);
+    w.k0 = t0 * p.tile_keys;
+    w.k1 = min(t1 * p.tile_keys, a.prefix_len);
+    at += t1 - t0;
+    return true;
+  }
+};
+
+// The piece of a block that takes a split of a sequence's own keys; row tiles
+// fastest, so that blocks that run together share keys.
+__device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
+  PaPiece w;
+  const PaOwn& o = a.own;
+  const int tile = i % o.row_tiles;
+  i /= o.row_tiles;
+  w.head = i % a.hkv;
+  i /= a.hkv;
+  w.seq = i / o.splits;
+  const int split = i - w.seq * o.splits;
+  w.row0 = tile * o.tile_rows;
+  w.rows = a.seq_rows.d;
+  w.part = a.prefix.parts + split;
+  // keys that the tile's last row sees
+  const int n = max(seq_len(a, w.seq), 0);
+  const int last = a.group(min(w.row0 + o.tile_rows, w.rows) - 1);  // its query
+  const int len = min(n, max(n - a.tq + last + 1, 0));
+  const int tiles = (len + o.tile_keys - 1) / o.tile_keys;
+  w.k0 = static_cast<int>(static_cast<long>(tiles) * split / o.splits) * o.tile_keys;
+  w.k1 = min(static_cast<int>(static_cast<long>(tiles) * (split + 1) / o.splits) * o.tile_keys, len);
   return w;
 }
 
@@ -163,7 +197,7 @@ __device__ __forceinline__ long key_offset(const PaArgs& a, const int* table, in
   }
   return page * a.page_stride + static_cast<long>(j - p * a.page_rows.d) * a.row_stride;
 }
-__device__ __forceinline__ const int* table_of(const PaArgs& a, const PaItem& w) {
+__device__ __forceinline__ const int* table_of(const PaArgs& a, const PaPiece& w) {
   return w.seq < 0 ? a.prefix_pages : a.pages + static_cast<long>(w.seq) * a.max_pages;
 }
 
