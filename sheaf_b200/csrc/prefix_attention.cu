@@ -245,10 +245,12 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   if (a.lse && lane == 0) a.lse[at] = m + logf(l);
 }
 
-// How the keys of both segments are cut.
+// Which kernel takes a segment, and how its keys are cut.
+enum Kernel { kSimt, kMma, kTc };
 struct Plan {
   PaPrefix prefix = {};
   PaOwn own = {};
+  Kernel prefix_kernel, own_kernel;
   int own_ctas = 0;
   long parts() const { return prefix.parts + own.splits; }
 };
@@ -257,28 +259,42 @@ long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long G = d.h_q / d.cache.n_heads, hkv = d.cache.n_heads;
-  const bool f32 = d.cache.elem == SB_ELEM_F32;
   const long prefix_rows = static_cast<long>(d.b) * d.tq * G, own_rows = d.tq * G;
-  const auto tile_rows = [&](long rows) { return f32 || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); };
-  const int tile_keys = f32 ? kKeys : 64;
-  p.prefix.tile_rows = tile_rows(prefix_rows);
-  p.own.tile_rows = tile_rows(own_rows);
-  p.prefix.tile_keys = p.own.tile_keys = tile_keys;
+  const auto choose = [&](long rows) {
+    if (d.cache.elem == SB_ELEM_F32) return kSimt;
+    return rows > 64 ? kTc : kMma;
+  };
+  const auto rows_of = [](Kernel k, long rows) {
+    if (k == kTc) return rows > 128 ? 256 : 128;
+    return k == kSimt || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  };
+  const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : kKeys); };
+  p.prefix_kernel = choose(prefix_rows);
+  p.own_kernel = choose(own_rows);
+  p.prefix.tile_rows = rows_of(p.prefix_kernel, prefix_rows);
+  p.own.tile_rows = rows_of(p.own_kernel, own_rows);
+  p.prefix.tile_keys = keys_of(p.prefix_kernel);
+  p.own.tile_keys = keys_of(p.own_kernel);
   p.prefix.row_tiles = static_cast<int>(ceil_div(prefix_rows, p.prefix.tile_rows));
   p.own.row_tiles = static_cast<int>(ceil_div(own_rows, p.own.tile_rows));
-  p.prefix.tiles = static_cast<int>(ceil_div(d.prefix_len, tile_keys));
-  const long own_tiles = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, tile_keys);
+  p.prefix.tiles = static_cast<int>(ceil_div(d.prefix_len, p.prefix.tile_keys));
+  const long own_tiles = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, p.own.tile_keys);
   const long prefix_work = hkv * p.prefix.row_tiles * p.prefix.tiles;
-  const long own_items = d.b * hkv * p.own.row_tiles;
-  // key tiles that a block takes: at least 2, and enough that all blocks fit
-  // two to an SM
-  const long quota = std::max(2L, ceil_div(prefix_work + own_items * own_tiles, 2L * num_sms_cached()));
-  if (quota > 0x7fffffffL) return false;
-  p.prefix.per_cta = static_cast<int>(quota);
-  p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, quota));
-  p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / quota + 2) : 0;
-  if (p.prefix.tiles > 0 && quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
-  p.own.splits = static_cast<int>(std::min(64L, ceil_div(own_tiles, quota)));
+  const long own_items = d.b * hkv * p.own.row_tiles, own_work = own_items * own_tiles;
+  // Key tiles that a block takes: at least 2, and enough that all blocks of a
+  // launch are resident at once, one (tcgen05) or two to an SM.
+  const bool together = p.prefix_kernel == p.own_kernel;
+  const auto quota = [&](Kernel k, long work) {
+    return std::max(2L, ceil_div(work, (k == kTc ? 1L : 2L) * num_sms_cached()));
+  };
+  const long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
+  const long own_quota = quota(p.own_kernel, own_work + (together ? prefix_work : 0));
+  if (prefix_quota > 0x7fffffffL) return false;
+  p.prefix.per_cta = static_cast<int>(prefix_quota);
+  p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, prefix_quota));
+  p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / prefix_quota + 2) : 0;
+  if (p.prefix.tiles > 0 && prefix_quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
+  p.own.splits = static_cast<int>(std::min(64L, ceil_div(own_tiles, own_quota)));
   if (p.parts() == 0) p.own.splits = 1;  // no keys at all: one empty part
   const long own_ctas = own_items * p.own.splits;
   if (own_ctas + p.prefix.ctas > 0x7fffffffL) return false;
@@ -315,6 +331,7 @@ size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
 }  // namespace
 
 int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
+int attn_tc(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
 
 size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {
   Plan p;
@@ -361,10 +378,15 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   a.err = err;
   const int hd = d.cache.head_dim;
   const bool f32 = d.cache.elem == SB_ELEM_F32;
-  int rc;
-  if (!f32)
-    rc = attn_mma(a, hd, a.prefix.ctas, p.own_ctas, s);
-  else
+  int rc = 0;
+  if (!f32) {
+    const bool prefix_tc = p.prefix_kernel == kTc && a.prefix.ctas > 0, own_tc = p.own_kernel == kTc;
+    const int mma_prefix = prefix_tc ? 0 : a.prefix.ctas, mma_own = own_tc ? 0 : p.own_ctas;
+    const int tc_prefix = prefix_tc ? a.prefix.ctas : 0, tc_own = own_tc ? p.own_ctas : 0;
+    // the two write parts of their own: the second starts beside the first
+    if (mma_prefix + mma_own > 0) rc = attn_mma(a, hd, mma_prefix, mma_own, s);
+    if (!rc && tc_prefix + tc_own > 0) rc = attn_tc(a, hd, tc_prefix, tc_own, mma_prefix + mma_own > 0, s);
+  } else
     rc = hd == 32 ? simt<32>(a, p.own_ctas, s) : (hd == 64 ? simt<64>(a, p.own_ctas, s) : simt<128>(a, p.own_ctas, s));
   if (rc || a.direct) return rc;
   return f32 ? join<float>(a, hd, s) : join<__nv_bfloat16>(a, hd, s);
