@@ -825,6 +825,21 @@ bool make_tma_3d_bf16(void* map, const void* base, long d0, long d1, long d2, lo
   return r == CUDA_SUCCESS;
 }
 
+// 4-D tiled map (128-byte swizzle) over [d3, d2, d1, d0] bf16 with byte
+// strides, boxes of box0 x 1 x box2 x 1; values past d0 read as zero.
+bool make_tma_4d_bf16(void* map, const void* base, const long (&d)[4], const long (&stride)[3], int box0, int box2) {
+  auto fn = get_encode_fn();
+  if (!fn || !base) return false;
+  cuuint64_t dims[4], strides[3];
+  for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(d[i]);
+  for (int i = 0; i < 3; ++i) strides[i] = static_cast<cuuint64_t>(stride[i]);
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(box0), 1, static_cast<cuuint32_t>(box2), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool make_tma_2d_f32(void* map, const void* base, long rows, long cols, long ld, int box_cols, int box_rows) {
   return make_map(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_cols,
                   box_rows);

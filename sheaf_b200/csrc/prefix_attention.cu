@@ -10,6 +10,7 @@
 namespace sb {
 
 int num_sms_cached();
+int warp_blocks_per_sm(int hd);
 
 namespace {
 
@@ -198,16 +199,20 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
   }
 }
 
-// A warp per row joins its partial results; a part that saw no key (l = 0)
-// left no output and is not read.
-template <typename T, int HD>
+// Joins a row's partial results with WPR warps, each taking every WPR-th part
+// in order, then the warps in order. A part that saw no key (l = 0) left no
+// output and is not read.
+template <typename T, int HD, int WPR>
 __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   constexpr int C = HD / 32;
-  pdl_wait();
+  __shared__ float sh_o[WPR > 1 ? 8 : 1][HD];
+  __shared__ float2 sh_ml[8];
   const long rows = static_cast<long>(a.b) * a.tq * a.hq;
-  const long at = static_cast<long>(blockIdx.x) * 8 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (at >= rows) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long at = WPR == 1 ? static_cast<long>(blockIdx.x) * 8 + warp : blockIdx.x;
+  const int first = WPR == 1 ? 0 : warp;
+  pdl_wait();
+  if (WPR == 1 && at >= rows) return;
   const long token = at / a.hq;
   const int h = static_cast<int>(at - token * a.hq);
   int n_prefix = 0;
@@ -218,25 +223,61 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   }
   const int parts = n_prefix + a.own.splits;
   const auto slot = [&](int p) { return (p < n_prefix ? p : a.prefix.parts + p - n_prefix) * rows + at; };
-  float m = -INFINITY;
-  for (int p = lane; p < parts; p += 32) {
-    const float2 ml = a.part_ml[slot(p)];
-    if (ml.y != 0.f) m = fmaxf(m, ml.x);
-  }
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  float l = 0.f, o[C];
+  float m = -INFINITY, l = 0.f, o[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[slot(p)];
-    if (ml.y == 0.f) continue;
-    const float f = expf(ml.x - m);
-    l = fmaf(ml.y, f, l);
-    const float* src = a.part_o + slot(p) * HD + lane * C;
+  // groups of U parts: their loads are in flight together
+  constexpr int U = 4;
+  for (int p0 = first; p0 < parts; p0 += U * WPR) {
+    float2 ml[U];
+    float v[U][C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = fmaf(src[c], f, o[c]);
+    for (int u = 0; u < U; ++u) {
+      const int p = p0 + u * WPR;
+      ml[u] = p < parts ? a.part_ml[slot(p)] : make_float2(-INFINITY, 0.f);
+      const float* src = a.part_o + slot(min(p, parts - 1)) * HD + lane * C;
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[u][c] = src[c];  // counts only where l is not 0
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ml[u].y != 0.f) mn = fmaxf(mn, ml[u].x);
+    const float f0 = l != 0.f ? expf(m - mn) : 0.f;
+    l *= f0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ml[u].y == 0.f) continue;
+      const float f = expf(ml[u].x - mn);
+      l = fmaf(ml[u].y, f, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(v[u][c], f, o[c]);
+    }
+    m = mn;
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) sh_o[warp][lane * C + c] = o[c];
+    if (lane == 0) sh_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp > 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w)
+      if (sh_ml[w].y != 0.f) m = fmaxf(m, sh_ml[w].x);
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      if (sh_ml[w].y == 0.f) continue;
+      const float f = expf(sh_ml[w].x - m);
+      l = fmaf(sh_ml[w].y, f, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(sh_o[w][lane * C + c], f, o[c]);
+    }
   }
   const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* out = static_cast<T*>(a.out) + token * a.ldo + static_cast<long>(h) * HD + lane * C;
@@ -245,8 +286,20 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   if (a.lse && lane == 0) a.lse[at] = m + logf(l);
 }
 
+// Rows of the tiled copies that follow a page table: the largest power of two
+// that divides a page, at most `most`; 0 where such a copy cannot (it would not
+// start on the swizzle's 8 rows, or the strides are none that a tensor map
+// takes).
+int tiled_rows(const sb_kv_cache& c, int most) {
+  const auto strides = [](int64_t s, int count) { return count == 1 || (s > 0 && s < (int64_t{1} << 38)); };
+  if (c.page_rows % 8 || !strides(c.page_stride, c.n_pages) || !strides(c.row_stride, c.page_rows) ||
+      !strides(c.head_stride, c.n_heads))
+    return 0;
+  return std::min(c.page_rows & -c.page_rows, most);
+}
+
 // Which kernel takes a segment, and how its keys are cut.
-enum Kernel { kSimt, kMma, kTc };
+enum Kernel { kSimt, kWarp, kMma, kTc };
 struct Plan {
   PaPrefix prefix = {};
   PaOwn own = {};
@@ -262,13 +315,14 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long prefix_rows = static_cast<long>(d.b) * d.tq * G, own_rows = d.tq * G;
   const auto choose = [&](long rows) {
     if (d.cache.elem == SB_ELEM_F32) return kSimt;
-    return rows > 64 ? kTc : kMma;
+    if (rows <= 16) return kWarp;
+    return rows > 64 && tiled_rows(d.cache, 128) ? kTc : kMma;
   };
   const auto rows_of = [](Kernel k, long rows) {
     if (k == kTc) return rows > 128 ? 256 : 128;
     return k == kSimt || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
   };
-  const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : kKeys); };
+  const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : (k == kWarp ? 16 : kKeys)); };
   p.prefix_kernel = choose(prefix_rows);
   p.own_kernel = choose(own_rows);
   p.prefix.tile_rows = rows_of(p.prefix_kernel, prefix_rows);
@@ -282,10 +336,11 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long prefix_work = hkv * p.prefix.row_tiles * p.prefix.tiles;
   const long own_items = d.b * hkv * p.own.row_tiles, own_work = own_items * own_tiles;
   // Key tiles that a block takes: at least 2, and enough that all blocks of a
-  // launch are resident at once, one (tcgen05) or two to an SM.
+  // launch are resident at once.
   const bool together = p.prefix_kernel == p.own_kernel;
   const auto quota = [&](Kernel k, long work) {
-    return std::max(2L, ceil_div(work, (k == kTc ? 1L : 2L) * num_sms_cached()));
+    const long blocks = k == kTc ? 1 : (k == kWarp ? warp_blocks_per_sm(d.cache.head_dim) : 2);
+    return std::max(k == kWarp ? 4L : 2L, ceil_div(work, blocks * num_sms_cached()));
   };
   const long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
   const long own_quota = quota(p.own_kernel, own_work + (together ? prefix_work : 0));
@@ -294,13 +349,27 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, prefix_quota));
   p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / prefix_quota + 2) : 0;
   if (p.prefix.tiles > 0 && prefix_quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
-  p.own.splits = static_cast<int>(std::min(64L, ceil_div(own_tiles, own_quota)));
+  p.own.splits = static_cast<int>(std::min(256L, ceil_div(own_tiles, own_quota)));
   if (p.parts() == 0) p.own.splits = 1;  // no keys at all: one empty part
   const long own_ctas = own_items * p.own.splits;
   if (own_ctas + p.prefix.ctas > 0x7fffffffL) return false;
   p.own_ctas = static_cast<int>(own_ctas);
   return true;
 }
+
+}  // namespace
+
+// Tensor map over the pages of k or v: [page][row][head][head_dim], boxes of
+// 64 values of a head in box_rows rows.
+bool cache_map(void* map, const void* base, const PaArgs& a, int hd) {
+  const long dims[4] = {hd, a.hkv, static_cast<long>(a.page_rows.d), a.n_pages};
+  // the stride of a dimension of one is free, but the map wants a usable one
+  const auto bytes = [&](long s, long count) { return count == 1 ? 16 * 16 : s * 2; };
+  const long strides[3] = {bytes(a.head_stride, dims[1]), bytes(a.row_stride, dims[2]), bytes(a.page_stride, dims[3])};
+  return make_tma_4d_bf16(map, base, dims, strides, 64, a.box_rows);
+}
+
+namespace {
 
 template <int HD>
 int simt(const PaArgs& a, int own_ctas, cudaStream_t s) {
@@ -318,12 +387,19 @@ int simt(const PaArgs& a, int own_ctas, cudaStream_t s) {
              : SB_OPERR_LAUNCH;
 }
 
+template <typename T, int HD>
+int join(const PaArgs& a, cudaStream_t s) {
+  const long rows = static_cast<long>(a.b) * a.tq * a.hq;
+  const bool wide = a.prefix.parts + a.own.splits > 8;
+  const dim3 grid(static_cast<unsigned>(wide ? rows : (rows + 7) / 8));
+  return launch_pdl(wide ? attn_join_kernel<T, HD, 8> : attn_join_kernel<T, HD, 1>, grid, dim3(256), 0, s, a) ==
+                 cudaSuccess
+             ? 0
+             : SB_OPERR_LAUNCH;
+}
 template <typename T>
 int join(const PaArgs& a, int hd, cudaStream_t s) {
-  const long rows = static_cast<long>(a.b) * a.tq * a.hq;
-  const dim3 grid(static_cast<unsigned>((rows + 7) / 8));
-  const auto k = hd == 32 ? attn_join_kernel<T, 32> : (hd == 64 ? attn_join_kernel<T, 64> : attn_join_kernel<T, 128>);
-  return launch_pdl(k, grid, dim3(256), 0, s, a) == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
+  return hd == 32 ? join<T, 32>(a, s) : (hd == 64 ? join<T, 64>(a, s) : join<T, 128>(a, s));
 }
 
 size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
@@ -331,6 +407,7 @@ size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
 }  // namespace
 
 int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
+int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_items, cudaStream_t s);
 int attn_tc(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
 
 size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {
@@ -372,6 +449,7 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   a.prefix = p.prefix;
   a.own = p.own;
   a.direct = p.parts() == 1;
+  a.box_rows = tiled_rows(d.cache, 128);
   const size_t rows = static_cast<size_t>(d.b) * d.tq * d.h_q;
   a.part_ml = static_cast<float2*>(ws);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align16(p.parts() * rows * sizeof(float2)));
@@ -380,12 +458,24 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   const bool f32 = d.cache.elem == SB_ELEM_F32;
   int rc = 0;
   if (!f32) {
-    const bool prefix_tc = p.prefix_kernel == kTc && a.prefix.ctas > 0, own_tc = p.own_kernel == kTc;
-    const int mma_prefix = prefix_tc ? 0 : a.prefix.ctas, mma_own = own_tc ? 0 : p.own_ctas;
-    const int tc_prefix = prefix_tc ? a.prefix.ctas : 0, tc_own = own_tc ? p.own_ctas : 0;
-    // the two write parts of their own: the second starts beside the first
-    if (mma_prefix + mma_own > 0) rc = attn_mma(a, hd, mma_prefix, mma_own, s);
-    if (!rc && tc_prefix + tc_own > 0) rc = attn_tc(a, hd, tc_prefix, tc_own, mma_prefix + mma_own > 0, s);
+    // A kernel takes both segments or one; parts of the two are apart, so a
+    // tcgen05 launch starts beside the one before it.
+    const auto of = [&](Kernel k, int& prefix, int& own) {
+      prefix = p.prefix_kernel == k ? a.prefix.ctas : 0;
+      own = p.own_kernel == k ? p.own_ctas : 0;
+      return prefix + own > 0;
+    };
+    int prefix, own;
+    bool before = false;
+    if (of(kWarp, prefix, own)) {
+      rc = attn_warp(a, hd, prefix, own, s);
+      before = true;
+    }
+    if (!rc && of(kMma, prefix, own)) {
+      rc = attn_mma(a, hd, prefix, own, s);
+      before = true;
+    }
+    if (!rc && of(kTc, prefix, own)) rc = attn_tc(a, hd, prefix, own, before, s);
   } else
     rc = hd == 32 ? simt<32>(a, p.own_ctas, s) : (hd == 64 ? simt<64>(a, p.own_ctas, s) : simt<128>(a, p.own_ctas, s));
   if (rc || a.direct) return rc;

@@ -87,6 +87,7 @@ struct PaArgs {
   // parts: the prefix's, then the own splits'
   float* part_o;
   float2* part_ml;
+  int box_rows;      // rows of a tiled copy: a power of two that divides a page
   bool direct;       // there is one part: results go straight to out, lse
   int* err;
 };
@@ -187,19 +188,25 @@ __device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
   return w;
 }
 
-// Element offset of key j of the segment (head 0).
-__device__ __forceinline__ long key_offset(const PaArgs& a, const int* table, int j) {
-  const int p = a.page_rows(j);
-  int page = table[p];
+// Page of the segment that holds its key j.
+__device__ __forceinline__ int page_of(const PaArgs& a, const int* table, int j) {
+  int page = table[a.page_rows(j)];
   if (page < 0 || page >= a.n_pages) {
     if (a.err) atomicExch(a.err, kErrIndex);
     page = 0;
   }
-  return page * a.page_stride + static_cast<long>(j - p * a.page_rows.d) * a.row_stride;
+  return page;
+}
+// Element offset of key j of the segment (head 0).
+__device__ __forceinline__ long key_offset(const PaArgs& a, const int* table, int j) {
+  const int row = j - static_cast<int>(a.page_rows(j) * a.page_rows.d);
+  return page_of(a, table, j) * a.page_stride + static_cast<long>(row) * a.row_stride;
 }
 __device__ __forceinline__ const int* table_of(const PaArgs& a, const PaPiece& w) {
   return w.seq < 0 ? a.prefix_pages : a.pages + static_cast<long>(w.seq) * a.max_pages;
 }
+
+bool cache_map(void* map, const void* base, const PaArgs& a, int hd);
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");

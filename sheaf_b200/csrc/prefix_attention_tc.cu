@@ -5,18 +5,22 @@
 //
 // A block takes up to 256 rows, two tiles of 128, against tiles of 128 keys;
 // 12 warps:
-//   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row. S is read from
-//             TMEM twice (maximum, then 2^(s - r)); P goes back to TMEM as
-//             bf16 over the columns of S it came from, the A operand of P V.
+//   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row, which holds its
+//             128 scores in registers; P goes back to TMEM as bf16 over the
+//             columns of S it came from, the A operand of P V.
 //             The reference r of a row's exponents rises only when a score
 //             passes it by 8, so O (in TMEM) is rescaled rarely.
 //   warp 8    TMEM owner, one thread issues the UMMAs: for row tile x
 //             S_x = Q_x K^T (128 x 128 x HD), O_x += P_x V (128 x HD x 128).
 //             While one row tile's softmax runs, the other's products do.
-//   warps 9-11  gather Q, K and V rows through the page tables with
-//             asynchronous 16-byte copies into 128-byte-swizzled tiles (a
-//             page may end anywhere in a tile, which a tiled bulk copy could
-//             not follow).
+//   warps 9, 10  copy K, V through the page tables: a tiled bulk copy for each
+//             run of rows that lies in one page whatever the tile's place (the
+//             largest power of two that divides the page), a lane each. One
+//             warp for both had K wait for room for V and took 5200 cycles a
+//             tile where two take TODO.
+//   warp 11   looks through the tiles of V in which a row stops (below).
+// The softmax warps gather their rows of Q, those of the next piece while the
+// last products of this one run.
 // TMEM: S_0, S_1 (128 columns each), O_0, O_1 (HD each).
 #include <algorithm>
 
@@ -31,10 +35,12 @@ namespace {
 
 constexpr int kRows = 128;  // rows of a tile
 constexpr int kKeys = 128;  // keys of a tile
-constexpr int kSoftWarps = 8, kLoadWarps = 3;  // 12 warps: 168 registers a thread
-constexpr int kThreads = 32 * (kSoftWarps + 1 + kLoadWarps);
+constexpr int kSoftWarps = 8;
+constexpr int kThreads = 32 * (kSoftWarps + 4);  // 168 registers a thread
+// Registers a thread: a softmax thread holds its row's 128 scores. Together
+// what the launch gave: 256 x 208 + 128 x 88 = 384 x 168.
+constexpr int kSoftRegs = 208, kOtherRegs = 88;
 constexpr int kAtom = 128 * 128;  // bytes of 128 rows x 64 values
-constexpr int kLag = 2;           // units of copies in flight behind the newest
 
 template <int HD>
 struct Tc {
@@ -47,10 +53,11 @@ struct Tc {
   static constexpr int kK = kQ + 2 * kTile;
   static constexpr int kV = kK + kStages * kTile;
   static constexpr int kOut = kV + kStages * kTile;
-  static constexpr int kOffset = kOut + kSoftWarps * kStageOut;  // long [2][kKeys]
-  static constexpr int kBad = kOffset + 2 * kKeys * 8;           // int [3 pieces][3][HD]
-  static constexpr int kBars = kBad + 9 * HD * 4;
-  static constexpr int kNumBars = 2 + 4 * kStages + 6;
+  static constexpr int kBad = kOut + kSoftWarps * kStageOut;  // int [3][HD]
+  static constexpr int kFound = kBad + 3 * HD * 4;  // int: the piece that kBad is about, plus one
+  static constexpr int kDone = kFound + 16;         // int [softmax warps]: pieces finished
+  static constexpr int kBars = kDone + 4 * kSoftWarps;
+  static constexpr int kNumBars = 2 + 5 * kStages + 6;
   static constexpr int kEnd = kBars + kNumBars * 8 + 32;
   static constexpr int kSmem = kEnd + 1024;
   static constexpr uint32_t kTmemO = 256;  // first column of O_0
@@ -64,10 +71,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void bar_named(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 // 16-byte chunk c of row r of a tile (K-major atoms of 64 values).
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -97,46 +108,71 @@ struct Pieces {
   }
 };
 
+// From this key on some row of the piece stops before the piece does. Such a
+// row must not meet the values behind its last key, even as 0 * NaN, so the
+// tiles of V from there on get their NaN and infinities taken out, to be added
+// to the rows that see them at the end. (A row that sees no key of the piece
+// is dropped by its l = 0.) All lanes of a warp get the answer.
+__device__ __forceinline__ int care_of(const PaArgs& a, const PaPiece& w, int tile_rows) {
+  int care = w.k1;
+  const int rows = min(tile_rows, w.rows - w.row0);
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {  // 256 rows; the loads are in flight together
+    const int i = min(n * 32 + static_cast<int>(threadIdx.x % 32), rows - 1);
+    const int seen = visible(a, w.seq < 0, row_of(a, w, w.row0 + i));
+    if (seen > w.k0) care = min(care, seen);
+  }
+  return __reduce_min_sync(0xffffffffu, care);
+}
+// Whether the values of tile j0 are looked through: a row stops inside it, or
+// the piece does (what lies behind is then whatever shared memory holds).
+__device__ __forceinline__ bool special(const PaPiece& w, int care, int j0) {
+  return care < j0 + kKeys;
+}
+
 // `early`: launched beside the kernel before it on the stream, whose own
 // predecessors have completed and which writes nothing that this one reads;
 // it is waited for at the end.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int prefix_ctas, int early) {
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                              const __grid_constant__ CUtensorMap tm_v, PaArgs a,
+                                                              int prefix_ctas, int early) {
   extern __shared__ uint8_t smem_raw[];
   using L = Tc<HD>;
   constexpr int ST = L::kStages;
   using bf = __nv_bfloat16;
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
+  uint64_t* q_full = bars;  // [2]
   uint64_t* k_full = bars + 2;
   uint64_t* k_empty = k_full + ST;
   uint64_t* v_full = k_empty + ST;
   uint64_t* v_empty = v_full + ST;
-  uint64_t* s_full = v_empty + ST;  // [2]
+  uint64_t* v_raw = v_empty + ST;   // a special tile of V has landed
+  uint64_t* s_full = v_raw + ST;    // [2]
   uint64_t* p_full = s_full + 2;    // [2]
   uint64_t* o_full = p_full + 2;    // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* care = reinterpret_cast<int*>(tmem_slot + 2);  // of the loaders
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, kLoadWarps);
-    mbar_init(q_empty, 1);
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&k_full[i], kLoadWarps);
+      mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], kLoadWarps);
+      mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_raw[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
     }
     *abort_flag = 0;
+    *reinterpret_cast<int*>(sm + L::kFound) = 0;
+    for (int i = 0; i < kSoftWarps; ++i) reinterpret_cast<int*>(sm + L::kDone)[i] = 0;
     fence_mbar_init();
   }
   if (!early) pdl_wait();
@@ -153,126 +189,120 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
   PaPiece w;
   const int tile_rows = static_cast<int>(blockIdx.x) < prefix_ctas ? a.prefix.tile_rows : a.own.tile_rows;
 
-  if (warp > kSoftWarps) {
-    // ---- gather ----------------------------------------------------------
-    const int tid = threadIdx.x - 32 * (kSoftWarps + 1);
-    constexpr int CH = HD / 8, N = kLoadWarps * 32;
-    long* offset = reinterpret_cast<long*>(sm + L::kOffset);
-    const uint32_t base = smem_u32(sm);
-    uint32_t unit = 0, signalled = 0;  // K and V tiles in turn
-    int piece = 0, slot = 0;
-    uint32_t q_units = 0;  // pieces whose Q is not announced yet
-    // The loaders go on after a wait that ran out (the waits then end at once),
-    // so that all their warps meet at the same barriers.
-    const auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (lane == 0) mbar_wait(bar, parity, a.err, abort_flag);
-      __syncwarp();
-    };
-    const auto signal = [&] {  // the oldest unit has landed for this thread
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        const uint32_t t = signalled >> 1;
-        if (!(signalled & 1)) {
-          if (q_units) mbar_arrive(q_full);
-          mbar_arrive(&k_full[t % ST]);
-        } else {
-          mbar_arrive(&v_full[t % ST]);
-        }
-      }
-      if (!(signalled & 1)) q_units = 0;
-      ++signalled;
-    };
-    while (pieces.next(a, w)) {
+  if (warp >= kSoftWarps) regs_down<kOtherRegs>();
+  if (warp == kSoftWarps + 1 || warp == kSoftWarps + 2) {
+    // ---- copies of K, V ----------------------------------------------------
+    const bool values = warp == kSoftWarps + 2;
+    const CUtensorMap* map = values ? &tm_v : &tm_k;
+    uint64_t* full = values ? v_full : k_full;
+    uint64_t* empty = values ? v_empty : k_empty;
+    const int boxes = kKeys / a.box_rows;  // of 64 values' width
+    const int row = lane % boxes * a.box_rows, atom = lane / boxes;  // this lane's box of a tile
+    const bool active = atom < L::kAtoms;
+    const uint32_t bytes = a.box_rows * 128;
+    const uint32_t to = smem_u32(sm) + (values ? L::kV : L::kK) + atom * kAtom + row * 128;
+    uint32_t t = 0;  // tiles so far
+    bool ok = true;
+    while (ok && pieces.next(a, w)) {
       if (w.k1 <= w.k0) continue;
-      const int n = (w.k1 - w.k0 + kKeys - 1) / kKeys;
-      // what is in flight is announced before waiting for the last piece's
-      // products, which need it
-      cp_async_wait<0>();
-      while (signalled < unit) signal();
-      if (piece > 0) wait(q_empty, (piece - 1) & 1);
-      int* bad = reinterpret_cast<int*>(sm + L::kBad) + (piece % 3) * 3 * HD;
-      const bool prefix = w.seq < 0;
       const int* table = table_of(a, w);
-      const bf* gk = static_cast<const bf*>(a.k) + static_cast<long>(w.head) * a.head_stride;
-      const bf* gv = static_cast<const bf*>(a.v) + static_cast<long>(w.head) * a.head_stride;
-      for (int i = tid; i < 3 * HD; i += N) bad[i] = 0x7fffffff;
-      if (tid == 0) *care = w.k1;
-      bar_named(1, N);
-      for (int i = tid; i < tile_rows; i += N) {
-        if (w.row0 + i >= w.rows) break;
-        const int seen = visible(a, prefix, row_of(a, w, w.row0 + i));
-        if (seen > w.k0 && seen < w.k1) atomicMin(care, seen);
-      }
-      // Q: rows past the segment's end are zero
-      for (int i = tid; i < tile_rows * CH; i += N) {
-        const int r = i / CH, c = i % CH;
-        const bool in = w.row0 + r < w.rows;
-        long at = 0;
-        if (in) {
-          const PaRow x = row_of(a, w, w.row0 + r);
-          at = x.token * a.ldq + static_cast<long>(x.h) * HD + c * 8;
+      int page = active && w.k0 + row < w.k1 ? page_of(a, table, w.k0 + row) : 0;
+      const int care = values ? care_of(a, w, tile_rows) : 0;
+      for (int j0 = w.k0; j0 < w.k1; j0 += kKeys, ++t) {
+        const bool mine = active && j0 + row < w.k1;
+        const int in_page = j0 + row - static_cast<int>(a.page_rows(j0 + row) * a.page_rows.d);
+        const uint32_t all = __popc(__ballot_sync(0xffffffffu, mine)) * bytes;
+        const int this_page = page;
+        if (active && j0 + kKeys + row < w.k1) page = page_of(a, table, j0 + kKeys + row);
+        const uint32_t st = t % ST;
+        if (t >= ST) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ((t / ST) & 1) ^ 1, a.err, abort_flag));
+          if (!ok) break;
         }
-        cp_async16(base + L::kQ + (r / kRows) * L::kTile + chunk_at(r % kRows, c), static_cast<const bf*>(a.q) + at, in);
+        uint64_t* bar = values && special(w, care, j0) ? &v_raw[st] : &full[st];
+        if (lane == 0) mbar_arrive_expect_tx(bar, all);
+        __syncwarp();
+        if (mine) tma_load_4d(to + st * L::kTile, map, bar, atom * 64, w.head, in_page, this_page);
       }
-      ++q_units;
-      const auto locate = [&](int to, int j0) {
-        for (int i = tid; i < kKeys; i += N)
-          if (j0 + i < w.k1) offset[to * kKeys + i] = key_offset(a, table, j0 + i);
-      };
-      locate(slot, w.k0);
-      bar_named(1, N);
-      const int ragged = *care;
-      for (int j = 0; j < n; ++j) {
-        const int j0 = w.k0 + j * kKeys;
-        locate(slot ^ 1, j0 + kKeys);
+    }
+    if (!ok) {  // copies in flight land before the block may end, or a second passes
+      __syncwarp();
+      const unsigned long long t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 1000000000ull) {
+      }
+    }
+  } else if (warp > kSoftWarps + 2) {
+    // ---- special tiles of V ------------------------------------------------
+    constexpr int CH = HD / 8;
+    uint32_t t = 0, raw[ST] = {};  // tiles so far, special ones of a stage
+    int piece = 0;
+    bool ok = true;
+    while (ok && pieces.next(a, w)) {
+      if (w.k1 <= w.k0) continue;
+      const int care = care_of(a, w, tile_rows);
+      for (int j0 = w.k0; j0 < w.k1; j0 += kKeys, ++t) {
+        if (!special(w, care, j0)) continue;
+        const uint32_t st = t % ST;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // K, then V
-          const uint32_t t = unit >> 1, st = t % ST;
-          if (t >= ST) wait(half ? &v_empty[st] : &k_empty[st], ((t / ST) & 1) ^ 1);
-          const uint32_t tile = base + (half ? L::kV : L::kK) + st * L::kTile;
-          const bf* src = half ? gv : gk;
-#pragma unroll 8
-          for (int i = tid; i < kKeys * CH; i += N) {
-            const int r = i / CH, c = i % CH;
-            const bool in = j0 + r < w.k1;
-            cp_async16(tile + chunk_at(r, c), src + (in ? offset[slot * kKeys + r] + c * 8 : 0), in);
+        for (int s = 0; s < ST; ++s)
+          if (static_cast<uint32_t>(s) == st) ok = mbar_wait(&v_raw[st], raw[s]++ & 1, a.err, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* tile = sm + L::kV + st * L::kTile;
+        const int rows = min(kKeys, w.k1 - j0);
+        // rows behind the piece's end, which nothing was copied to, are zero
+        for (int i = rows * CH + lane; i < kKeys * CH; i += 32)
+          *reinterpret_cast<uint4*>(tile + chunk_at(i / CH, i % CH)) = make_uint4(0u, 0u, 0u, 0u);
+        if (care < j0 + rows) {
+          const auto odd = [](uint32_t x) {  // one of two bf16 is no number
+            return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+          };
+          bool any = false;
+#pragma unroll 4
+          for (int i = lane; i < rows * CH; i += 32) {
+            const uint4 u = *reinterpret_cast<const uint4*>(tile + chunk_at(i / CH, i % CH));
+            any |= odd(u.x) || odd(u.y) || odd(u.z) || odd(u.w);
           }
-          cp_async_commit();
-          if (half && ragged < min(j0 + kKeys, w.k1)) {
-            // some row stops inside this tile: values that it must not meet
-            // are taken out, each thread its own copies
-            cp_async_wait<0>();
-            for (int i = tid; i < kKeys * CH; i += N) {
+          if (__any_sync(0xffffffffu, any)) {
+            int* bad = reinterpret_cast<int*>(sm + L::kBad);
+            volatile int* found = reinterpret_cast<volatile int*>(sm + L::kFound);
+            volatile int* finished = reinterpret_cast<volatile int*>(sm + L::kDone);
+            if (*found != piece + 1) {  // the first of the piece: the pieces before are read to the end
+              const unsigned long long t0 = global_timer_ns();
+              while (!__all_sync(0xffffffffu, lane >= kSoftWarps || finished[lane] >= piece)) {
+                if (global_timer_ns() - t0 > kWaitLimitNs) {
+                  if (a.err) atomicExch(a.err, kErrBarrierTimeout);
+                  *abort_flag = 1;
+                  break;
+                }
+              }
+              for (int i = lane; i < 3 * HD; i += 32) bad[i] = 0x7fffffff;
+              __syncwarp();
+              if (lane == 0) *found = piece + 1;
+              __syncwarp();
+            }
+            for (int i = lane; i < rows * CH; i += 32) {
               const int r = i / CH, c = i % CH;
-              uint4* p = reinterpret_cast<uint4*>(sm + L::kV + st * L::kTile + chunk_at(r, c));
+              uint4* p = reinterpret_cast<uint4*>(tile + chunk_at(r, c));
               const uint4 u = *p;
               uint32_t x[4] = {u.x, u.y, u.z, u.w};
-              bool any = false;
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const uint32_t b = (x[e / 2] >> (16 * (e % 2))) & 0xffffu;
                 if ((b & 0x7f80u) != 0x7f80u) continue;
-                any = true;
                 x[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
                 atomicMin(&bad[((b & 0x7fu) ? 0 : (b >> 15 ? 2 : 1)) * HD + c * 8 + e], j0 + r);
               }
-              if (any) *p = make_uint4(x[0], x[1], x[2], x[3]);
+              *p = make_uint4(x[0], x[1], x[2], x[3]);
             }
           }
-          ++unit;
-          if (unit - signalled > kLag) {
-            cp_async_wait<kLag>();
-            signal();
-          }
         }
-        slot ^= 1;
-        bar_named(1, N);  // offsets of the next tile
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
       }
       ++piece;
     }
-    cp_async_wait<0>();
-    while (signalled < unit) signal();
   } else if (warp == kSoftWarps) {
     // ---- products --------------------------------------------------------
     if (lane == 0) {
@@ -281,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
       const uint32_t base = smem_u32(sm);
       uint32_t c = 0;             // key tiles so far
       uint32_t done[2] = {0, 0};  // of each row tile, which a piece may lack
-      int piece = 0;
+      uint32_t begun[2] = {0, 0};  // pieces
       bool ok = true;
       while (ok && pieces.next(a, w)) {
         if (w.k1 <= w.k0) continue;
@@ -300,11 +330,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
           }
           umma_commit(&s_full[x]);
         };
-        if (!wait(q_full, piece & 1) || !wait(&k_full[c % ST], (c / ST) & 1)) break;
-        tc_fence_after();
-        for (int x = 0; x < tiles; ++x) scores(x, c);
+        if (!wait(&k_full[c % ST], (c / ST) & 1)) break;
+        for (int x = 0; x < tiles; ++x) {
+          if (!wait(&q_full[x], begun[x]++ & 1)) break;
+          tc_fence_after();
+          scores(x, c);
+        }
+        if (!ok) break;
         umma_commit(&k_empty[c % ST]);
-        if (n == 1) umma_commit(q_empty);
         for (int j = 0; j < n && ok; ++j, ++c) {
           const uint32_t st = c % ST;
           if (!wait(&v_full[st], (c / ST) & 1)) break;
@@ -328,16 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
           }
           if (!ok) break;
           umma_commit(&v_empty[st]);
-          if (j + 1 < n) {
-            umma_commit(&k_empty[(c + 1) % ST]);
-            if (j + 2 == n) umma_commit(q_empty);
-          }
+          if (j + 1 < n) umma_commit(&k_empty[(c + 1) % ST]);
         }
-        ++piece;
       }
       // no commit may arrive on this block's barriers after it has exited
-      if (ok && piece > 0) {
-        mbar_wait(q_empty, (piece - 1) & 1, a.err, abort_flag);
+      if (ok) {
         for (uint32_t t = c >= ST ? c - ST : 0; t < c; ++t) {
           mbar_wait(&k_empty[t % ST], (t / ST) & 1, a.err, abort_flag);
           mbar_wait(&v_empty[t % ST], (t / ST) & 1, a.err, abort_flag);
@@ -347,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
     __syncwarp();
   } else {
     // ---- softmax ---------------------------------------------------------
+    regs_up<kSoftRegs>();
     const int x = warp / 4, quarter = warp % 4;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lanes + x * 128, tO = tmem + lanes + L::kTmemO + x * HD;
@@ -360,43 +389,86 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
       tc_fence_after();
       return ok;
     };
-    while (ok && pieces.next(a, w)) {
-      const bool prefix = w.seq < 0;
-      const bool work = w.k1 > w.k0;
-      const int n = work ? (w.k1 - w.k0 + kKeys - 1) / kKeys : 0;
-      const int i = w.row0 + x * kRows + quarter * 32 + lane;
-      const bool mine = x * kRows < tile_rows && i < w.rows;
-      int seen = w.k1;
-      long at = -1, out_at = 0;  // row among the results, offset of its output
-      if (mine) {
-        const PaRow r = row_of(a, w, i);
-        seen = min(visible(a, prefix, r), w.k1);
-        at = r.token * a.hq + r.h;
-        out_at = r.token * a.ldo + static_cast<long>(r.h) * HD;
+    // this thread's row of a piece
+    struct Mine {
+      bool in, present;  // has a row; the row tile has
+      int seen;
+      long at, out_at;   // among the results; offset of its output
+    };
+    const auto row_in = [&](const PaPiece& p) {
+      Mine m;
+      const int i = p.row0 + x * kRows + quarter * 32 + lane;
+      m.present = x == 0 || (tile_rows > kRows && p.row0 + kRows < p.rows);
+      m.in = m.present && i < p.rows;
+      m.seen = p.k1;
+      m.at = 0;
+      m.out_at = 0;
+      long q_at = -1;
+      if (m.in) {
+        const PaRow r = row_of(a, p, i);
+        m.seen = min(visible(a, p.seq < 0, r), p.k1);
+        m.at = r.token * a.hq + r.h;
+        m.out_at = r.token * a.ldo + static_cast<long>(r.h) * HD;
+        q_at = r.token * a.ldq + static_cast<long>(r.h) * HD;
       }
+      // this warp's rows of Q; rows past the segment's end are zero. The
+      // row tile's last scores are done: Q is free.
+      if (m.present && p.k1 > p.k0) {
+        constexpr int CH = HD / 8, RPI = 32 / CH;  // rows an instruction
+#pragma unroll
+        for (int n = 0; n < 32 / RPI; ++n) {
+          const int r = n * RPI + lane / CH, ch = lane % CH;
+          const long from = __shfl_sync(0xffffffffu, q_at, r);
+          cp_async16(smem_u32(sm) + L::kQ + x * L::kTile + chunk_at(quarter * 32 + r, ch),
+                     static_cast<const bf*>(a.q) + (from < 0 ? 0 : from + ch * 8), from >= 0);
+        }
+      }
+      cp_async_commit();
+      return m;
+    };
+    const auto announce_q = [&](const Mine& m, const PaPiece& p) {
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && m.present && p.k1 > p.k0) mbar_arrive(&q_full[x]);
+    };
+    PaPiece next_w;
+    bool more = pieces.next(a, next_w);
+    Mine next_mine = {};
+    if (more) {
+      next_mine = row_in(next_w);
+      announce_q(next_mine, next_w);
+    }
+    while (ok && more) {
+      w = next_w;
+      const Mine mine = next_mine;
+      const bool work = w.k1 > w.k0, present = mine.present;
+      const int n = work ? (w.k1 - w.k0 + kKeys - 1) / kKeys : 0;
+      const int seen = mine.seen;
       const int least = __reduce_min_sync(0xffffffffu, seen);
-      const bool present = x == 0 || (tile_rows > kRows && w.row0 + kRows < w.rows);
       float ref = -INFINITY, l = 0.f;
       if (present) {
         for (int j = 0; j < n; ++j, ++c) {
           const int j0 = w.k0 + j * kKeys;
           if (!wait(&s_full[x], c & 1)) break;
           const bool part = j0 + kKeys > least;  // some row stops in this tile
-          float mx = -INFINITY;
+          uint32_t v[4][32];  // this row's scores
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            uint32_t v[32];
-            tmem_ld32(tS + cc * 32, v);
-            tmem_wait_ld();
-            if (part) {
+          for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, v[cc]);
+          tmem_wait_ld();
+          if (part) {
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
               for (int t = 0; t < 32; ++t)
-                if (j0 + cc * 32 + t < seen) mx = fmaxf(mx, __uint_as_float(v[t]));
-            } else {
-#pragma unroll
-              for (int t = 0; t < 32; ++t) mx = fmaxf(mx, __uint_as_float(v[t]));
-            }
+                if (j0 + cc * 32 + t >= seen) v[cc][t] = __float_as_uint(-INFINITY);
           }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int t = 0; t < 32; ++t)
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) m4[cc] = fmaxf(m4[cc], __uint_as_float(v[cc][t]));
+          float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           mx *= sl;
           if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
             const float to = fmaxf(ref, mx);
@@ -407,69 +479,74 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
               if (!wait(&o_full[x], (c - 1) & 1)) break;
 #pragma unroll
               for (int cc = 0; cc < HD / 16; ++cc) {
-                uint32_t v[16];
-                tmem_ld16(tO + cc * 16, v);
+                uint32_t u[16];
+                tmem_ld16(tO + cc * 16, u);
                 tmem_wait_ld();
 #pragma unroll
-                for (int t = 0; t < 16; ++t) v[t] = __float_as_uint(__uint_as_float(v[t]) * f);
-                tmem_st16(tO + cc * 16, v);
+                for (int t = 0; t < 16; ++t) u[t] = __float_as_uint(__uint_as_float(u[t]) * f);
+                tmem_st16(tO + cc * 16, u);
               }
               tmem_wait_st();
             }
           }
           const float sub = ref == -INFINITY ? 0.f : ref;
-          float2 sum = make_float2(0.f, 0.f);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 sl2 = make_float2(sl, sl), sub2 = make_float2(-sub, -sub);
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
-            uint32_t v[32], pk[16];
-            tmem_ld32(tS + cc * 32, v);
-            tmem_wait_ld();
+            uint32_t pk[16];
 #pragma unroll
             for (int t = 0; t < 32; t += 2) {
               const float2 y =
-                  __ffma2_rn(make_float2(__uint_as_float(v[t]), __uint_as_float(v[t + 1])), sl2, sub2);
-              float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-              if (part) {
-                if (j0 + cc * 32 + t >= seen) p.x = 0.f;
-                if (j0 + cc * 32 + t + 1 >= seen) p.y = 0.f;
-              }
-              sum = __fadd2_rn(sum, p);
+                  __ffma2_rn(make_float2(__uint_as_float(v[cc][t]), __uint_as_float(v[cc][t + 1])), sl2, sub2);
+              const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+              sum[(t / 2) & 1] = __fadd2_rn(sum[(t / 2) & 1], p);
               pk[t / 2] = pack_bf16x2(p.x, p.y);
             }
             tmem_st16(tS + cc * 16, pk);
           }
-          l += sum.x + sum.y;
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[x]);
         }
         if (!ok) break;
-        if (n > 0 && !wait(&o_full[x], (c - 1) & 1)) break;
       }
+      more = pieces.next(a, next_w);
+      if (more) next_mine = row_in(next_w);
+      if (present && n > 0 && !wait(&o_full[x], (c - 1) & 1)) break;
       const float nat = ref * 0.6931471805599453f;  // natural units outside
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      if (mine) {
+      const long part_at = static_cast<long>(w.part) * a.b * a.tq * a.hq + mine.at;
+      if (mine.in) {
         if (a.direct) {
-          if (a.lse) a.lse[at] = nat + logf(l);
+          if (a.lse) a.lse[mine.at] = nat + logf(l);
         } else {
-          a.part_ml[static_cast<long>(w.part) * a.b * a.tq * a.hq + at] = make_float2(nat, l);
+          a.part_ml[part_at] = make_float2(nat, l);
         }
       }
       // rows leave through shared memory, 64 bytes of 8 rows a store
-      const int* bad = reinterpret_cast<const int*>(sm + L::kBad) + (piece % 3) * 3 * HD;
       if (present && (n > 0 || a.direct)) {
-        const long row_at = a.direct ? out_at : (static_cast<long>(w.part) * a.b * a.tq * a.hq + at) * HD;
-#pragma unroll 1
+        const bool some = n > 0 && *reinterpret_cast<volatile const int*>(sm + L::kFound) == piece + 1;
+        const int* bad = reinterpret_cast<const int*>(sm + L::kBad);
+        const long row_at = !mine.in || (!a.direct && l == 0.f) ? -1 : (a.direct ? mine.out_at : part_at * HD);
+        const float scale = a.direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+        long their_at[4];
+        float their_scale[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          their_at[k] = __shfl_sync(0xffffffffu, row_at, 8 * k + lane / 4);
+          their_scale[k] = __shfl_sync(0xffffffffu, scale, 8 * k + lane / 4);
+        }
+#pragma unroll
         for (int cc = 0; cc < HD / 16; ++cc) {
           uint32_t v[16];
-          if (n > 0) {
-            tmem_ld16(tO + cc * 16, v);
-            tmem_wait_ld();
-          } else {
+          tmem_ld16(tO + cc * 16, v);
+          tmem_wait_ld();
+          if (some && l != 0.f) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) v[t] = 0u;
+            for (int t = 0; t < 16; ++t)
+              v[t] = __float_as_uint(__uint_as_float(v[t]) + taken_out<HD>(bad, cc * 16 + t, seen));
           }
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -478,35 +555,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(PaArgs a, int pref
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int r = 8 * k + lane / 4, ch = lane % 4;
+            const int r = 8 * k + lane / 4, ch = lane % 4, col = cc * 16 + ch * 4;
             const uint4 u = ld_shared_v4(out_tile + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
-            const bool theirs = __shfl_sync(0xffffffffu, static_cast<int>(mine), r);
-            const float their_l = __shfl_sync(0xffffffffu, l, r);
-            const float their_inv = __shfl_sync(0xffffffffu, inv, r);
-            const int their_seen = __shfl_sync(0xffffffffu, seen, r);
-            const long their_at = __shfl_sync(0xffffffffu, row_at, r);
-            if (!theirs) continue;
-            float o[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
-            const int col = cc * 16 + ch * 4;
-            if (their_l != 0.f && n > 0) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[e] += taken_out<HD>(bad, col + e, their_seen);
-            }
+            if (their_at[k] < 0) continue;
             if (a.direct) {
-              if (their_l == 0.f) o[0] = o[1] = o[2] = o[3] = 0.f;
-              *reinterpret_cast<uint2*>(static_cast<bf*>(a.out) + their_at + col) =
-                  make_uint2(pack_bf16x2(o[0] * their_inv, o[1] * their_inv),
-                             pack_bf16x2(o[2] * their_inv, o[3] * their_inv));
-            } else if (their_l != 0.f) {
-              *reinterpret_cast<float4*>(a.part_o + their_at + col) = make_float4(o[0], o[1], o[2], o[3]);
+              const float f = their_scale[k];
+              uint2 o = make_uint2(pack_bf16x2(__uint_as_float(u.x) * f, __uint_as_float(u.y) * f),
+                                   pack_bf16x2(__uint_as_float(u.z) * f, __uint_as_float(u.w) * f));
+              if (f == 0.f) o = make_uint2(0u, 0u);  // a row that saw nothing
+              *reinterpret_cast<uint2*>(static_cast<bf*>(a.out) + their_at[k] + col) = o;
+            } else {
+              *reinterpret_cast<uint4*>(a.part_o + their_at[k] + col) = u;
             }
           }
           __syncwarp();
         }
       }
       tc_fence_before();  // O is read before the next piece's P is announced
-      if (work) ++piece;
+      if (more) announce_q(next_mine, next_w);
+      if (work) {
+        ++piece;
+        __syncwarp();
+        if (lane == 0) reinterpret_cast<volatile int*>(sm + L::kDone)[warp] = piece;
+      }
     }
+    cp_async_wait<0>();
   }
 
   if (early) pdl_wait();
@@ -527,9 +600,10 @@ int launch(const PaArgs& a, int prefix_ctas, int own_ctas, bool early, cudaStrea
       return SB_OPERR_LAUNCH;
     attr = true;
   }
-  // an early launch is one that the launch mask lets overlap; else the stream's order holds
+  alignas(64) CUtensorMap tk, tv;
+  if (!cache_map(&tk, a.k, a, HD) || !cache_map(&tv, a.v, a, HD)) return SB_OPERR_TMA;
   return launch_pdl(attn_tc_kernel<HD>, dim3(static_cast<unsigned>(prefix_ctas) + own_ctas), dim3(kThreads),
-                    Tc<HD>::kSmem, s, a, prefix_ctas, early ? 1 : 0) == cudaSuccess
+                    Tc<HD>::kSmem, s, tk, tv, a, prefix_ctas, early ? 1 : 0) == cudaSuccess
              ? 0
              : SB_OPERR_LAUNCH;
 }
