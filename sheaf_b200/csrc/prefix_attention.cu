@@ -344,7 +344,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   };
   const long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
   const long own_quota = quota(p.own_kernel, own_work + (together ? prefix_work : 0));
-  if (prefix_quota > 0x7fffffffL) return false;
+  if (prefix_work + prefix_quota > 0x7fffffffL) return false;  // counted in 32 bits
   p.prefix.per_cta = static_cast<int>(prefix_quota);
   p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, prefix_quota));
   p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / prefix_quota + 2) : 0;

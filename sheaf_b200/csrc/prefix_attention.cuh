@@ -47,11 +47,13 @@ struct PaPrefix {
   int tile_rows, tile_keys;
   int tiles, per_cta, ctas;
   int parts;      // most parts an item has
+  // (all key tiles together stay below 2^31)
   __host__ __device__ __forceinline__ int first(int item) const {
-    return static_cast<int>(static_cast<long>(item) * tiles / per_cta);
+    return static_cast<uint32_t>(item * tiles) / static_cast<uint32_t>(per_cta);
   }
   __host__ __device__ __forceinline__ int parts_of(int item) const {
-    return static_cast<int>((static_cast<long>(item + 1) * tiles - 1) / per_cta) - first(item) + 1;
+    return static_cast<int>(static_cast<uint32_t>((item + 1) * tiles - 1) / static_cast<uint32_t>(per_cta)) -
+           first(item) + 1;
   }
 };
 // The sequences' own keys: items (sequence, key head, tile of rows), each cut
@@ -141,25 +143,28 @@ __device__ __forceinline__ int visible(const PaArgs& a, bool prefix, const PaRow
 
 // The pieces of a block that takes a run of the prefix's key tiles.
 struct PaRun {
-  long at, end;
+  int item, tile, left;  // the next key tile and how many are left
   __device__ __forceinline__ PaRun(const PaPrefix& p, int hkv, int cta) {
-    at = static_cast<long>(cta) * p.per_cta;
-    end = min(at + p.per_cta, static_cast<long>(hkv) * p.row_tiles * p.tiles);
+    const uint32_t at = static_cast<uint32_t>(cta) * static_cast<uint32_t>(p.per_cta);
+    const uint32_t all = static_cast<uint32_t>(hkv) * p.row_tiles * p.tiles;
+    left = at < all ? static_cast<int>(min(all - at, static_cast<uint32_t>(p.per_cta))) : 0;
+    item = p.tiles ? at / static_cast<uint32_t>(p.tiles) : 0;
+    tile = static_cast<int>(at - static_cast<uint32_t>(item) * p.tiles);
   }
   __device__ __forceinline__ bool next(const PaArgs& a, int cta, PaPiece& w) {
-    if (at >= end) return false;
+    if (left <= 0) return false;
     const PaPrefix& p = a.prefix;
-    const int item = static_cast<int>(at / p.tiles);
-    const int t0 = static_cast<int>(at - static_cast<long>(item) * p.tiles);
-    const int t1 = static_cast<int>(min(end - static_cast<long>(item) * p.tiles, static_cast<long>(p.tiles)));
+    const int n = min(left, p.tiles - tile);
     w.seq = -1;
-    w.head = item / p.row_tiles;
+    w.head = static_cast<uint32_t>(item) / static_cast<uint32_t>(p.row_tiles);
     w.row0 = (item - w.head * p.row_tiles) * p.tile_rows;
     w.rows = a.b * a.seq_rows.d;
     w.part = cta - p.first(item);
-    w.k0 = t0 * p.tile_keys;
-    w.k1 = min(t1 * p.tile_keys, a.prefix_len);
-    at += t1 - t0;
+    w.k0 = tile * p.tile_keys;
+    w.k1 = min((tile + n) * p.tile_keys, a.prefix_len);
+    left -= n;
+    tile = 0;
+    ++item;
     return true;
   }
 };

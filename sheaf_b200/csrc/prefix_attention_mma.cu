@@ -24,7 +24,8 @@
 namespace sb {
 
 int num_sms_cached();
-constexpr int kWarpStageBytes = 4 * 2 * 16 * 2;  // of its ring, per value of a head
+constexpr int kWarpStages = 3;
+constexpr int kWarpStageBytes = kWarpStages * 2 * 16 * 2;  // of its ring, per value of a head
 // Blocks of the one-warp kernel that shared memory lets an SM hold (228 KB,
 // 1 KB a block to the system; at most 16, which keep enough in flight).
 int warp_blocks_per_sm(int hd) { return std::min(16, 228 * 1024 / (kWarpStageBytes * hd + 12 * hd + 1024)); }
@@ -386,7 +387,6 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(P
 // head) keep the SM's copies in flight. A block takes a run of the prefix, or
 // own pieces blockIdx, blockIdx + blocks, ..; the ring runs on into the next
 // piece, whose first copies are in flight while this one ends.
-constexpr int kWarpStages = 4;
 template <int HD>
 struct WarpShared {
   __nv_bfloat16 kv[kWarpStages][2][16 * HD];

@@ -5,11 +5,10 @@
 //
 // A block takes up to 256 rows, two tiles of 128, against tiles of 128 keys;
 // 12 warps:
-//   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row, which holds its
-//             128 scores in registers; P goes back to TMEM as bf16 over the
-//             columns of S it came from, the A operand of P V.
-//             The reference r of a row's exponents rises only when a score
-//             passes it by 8, so O (in TMEM) is rescaled rarely.
+//   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row; P goes back to TMEM as bf16 over the
+//             columns of S it came from, the A operand of P V. The reference
+//             r of a row's exponents 2^(s - r) rises only when their sum over a
+//             tile passes 2^15, so O (in TMEM) is rescaled rarely.
 //   warp 8    TMEM owner, one thread issues the UMMAs: for row tile x
 //             S_x = Q_x K^T (128 x 128 x HD), O_x += P_x V (128 x HD x 128).
 //             While one row tile's softmax runs, the other's products do.
@@ -305,74 +304,76 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
   } else if (warp == kSoftWarps) {
     // ---- products --------------------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t idS = make_idesc_bf16(128, 128, false, false);
-      constexpr uint32_t idO = make_idesc_bf16(128, HD, false, true);
-      const uint32_t base = smem_u32(sm);
-      uint32_t c = 0;             // key tiles so far
-      uint32_t done[2] = {0, 0};  // of each row tile, which a piece may lack
-      uint32_t begun[2] = {0, 0};  // pieces
-      bool ok = true;
-      while (ok && pieces.next(a, w)) {
-        if (w.k1 <= w.k0) continue;
-        const int n = (w.k1 - w.k0 + kKeys - 1) / kKeys;
-        const int tiles = (tile_rows > kRows && w.row0 + kRows < w.rows) ? 2 : 1;
-        const auto wait = [&](uint64_t* bar, uint32_t parity) {
-          ok = mbar_wait(bar, parity, a.err, abort_flag);
-          return ok;
-        };
-        const auto scores = [&](int x, uint32_t t) {
-          const uint32_t q = base + L::kQ + x * L::kTile, k = base + L::kK + (t % ST) * L::kTile;
+    // The whole warp runs this with the same values and one lane issues, so
+    // that the descriptors live in uniform registers; a step's descriptor is
+    // the tile's plus a constant.
+    constexpr uint32_t idS = make_idesc_bf16(128, 128, false, false);
+    constexpr uint32_t idO = make_idesc_bf16(128, HD, false, true);
+    constexpr uint32_t kStep = L::kTile >> 4;
+    const uint32_t base = smem_u32(sm);
+    const uint64_t dq = make_sw128_desc(base + L::kQ, 16, 1024), dk = make_sw128_desc(base + L::kK, 16, 1024);
+    const uint64_t dv = make_sw128_desc(base + L::kV, kAtom, 1024);
+    const bool one = elect_one_lane();
+    uint32_t c = 0, kst = 0, kph = 0, vst = 0, vph = 0;  // key tiles so far; stages and their phases
+    uint32_t done[2] = {0, 0};   // key tiles of each row tile, which a piece may lack
+    uint32_t begun[2] = {0, 0};  // pieces
+    bool ok = true;
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, abort_flag));
+      tc_fence_after();
+      return ok;
+    };
+    const auto scores = [&](int x) {
+      if (one) {
+        const uint64_t q = dq + x * kStep, k = dk + kst * kStep;
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t at = (kk >> 2) * kAtom + (kk & 3) * 32;
-            umma_f16(tmem + x * 128, make_sw128_desc(q + at, 16, 1024), make_sw128_desc(k + at, 16, 1024), idS, kk > 0);
-          }
-          umma_commit(&s_full[x]);
-        };
-        if (!wait(&k_full[c % ST], (c / ST) & 1)) break;
-        for (int x = 0; x < tiles; ++x) {
-          if (!wait(&q_full[x], begun[x]++ & 1)) break;
-          tc_fence_after();
-          scores(x, c);
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t at = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
+          umma_f16(tmem + x * 128, q + at, k + at, idS, kk > 0);
         }
-        if (!ok) break;
-        umma_commit(&k_empty[c % ST]);
-        for (int j = 0; j < n && ok; ++j, ++c) {
-          const uint32_t st = c % ST;
-          if (!wait(&v_full[st], (c / ST) & 1)) break;
-          const uint32_t v = base + L::kV + st * L::kTile;
-          for (int x = 0; x < tiles; ++x) {
-            if (!wait(&p_full[x], done[x] & 1)) break;
-            ++done[x];
-            tc_fence_after();
+        umma_commit(&s_full[x]);
+      }
+    };
+    while (ok && pieces.next(a, w)) {
+      if (w.k1 <= w.k0) continue;
+      const int n = (w.k1 - w.k0 + kKeys - 1) / kKeys;
+      const int tiles = (tile_rows > kRows && w.row0 + kRows < w.rows) ? 2 : 1;
+      if (!wait(&k_full[kst], kph)) break;
+      for (int x = 0; x < tiles; ++x) {
+        if (!wait(&q_full[x], begun[x]++ & 1)) break;
+        scores(x);
+      }
+      if (!ok) break;
+      for (int j = 0; j < n; ++j, ++c) {
+        if (one) umma_commit(&k_empty[kst]);
+        kst = kst + 1 == ST ? 0 : kst + 1;
+        kph ^= kst == 0;
+        if (!wait(&v_full[vst], vph)) break;
+        const uint64_t v = dv + vst * kStep;
+        for (int x = 0; x < tiles; ++x) {
+          if (!wait(&p_full[x], done[x]++ & 1)) break;
+          if (one) {
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk)
-              umma_f16_tmem_a(tmem + L::kTmemO + x * HD, tmem + x * 128 + kk * 8,
-                              make_sw128_desc(v + kk * 2048, kAtom, 1024), idO, (j > 0 || kk > 0) ? 1u : 0u);
+              umma_f16_tmem_a(tmem + L::kTmemO + x * HD, tmem + x * 128 + kk * 8, v + ((kk * 2048) >> 4), idO,
+                              (j > 0 || kk > 0) ? 1u : 0u);
             umma_commit(&o_full[x]);
-            if (j + 1 < n) {
-              if (x == 0) {
-                if (!wait(&k_full[(c + 1) % ST], ((c + 1) / ST) & 1)) break;
-                tc_fence_after();
-              }
-              scores(x, c + 1);
-            }
           }
-          if (!ok) break;
-          umma_commit(&v_empty[st]);
-          if (j + 1 < n) umma_commit(&k_empty[(c + 1) % ST]);
+          if (j + 1 < n) {
+            if (x == 0 && !wait(&k_full[kst], kph)) break;
+            scores(x);
+          }
         }
-      }
-      // no commit may arrive on this block's barriers after it has exited
-      if (ok) {
-        for (uint32_t t = c >= ST ? c - ST : 0; t < c; ++t) {
-          mbar_wait(&k_empty[t % ST], (t / ST) & 1, a.err, abort_flag);
-          mbar_wait(&v_empty[t % ST], (t / ST) & 1, a.err, abort_flag);
-        }
+        if (!ok) break;
+        if (one) umma_commit(&v_empty[vst]);
+        vst = vst + 1 == ST ? 0 : vst + 1;
+        vph ^= vst == 0;
       }
     }
-    __syncwarp();
+    // no commit may arrive on this block's barriers after it has exited
+    if (ok)
+      for (uint32_t t = c >= ST ? c - ST : 0; t < c; ++t)
+        if (!wait(&k_empty[t % ST], (t / ST) & 1) || !wait(&v_empty[t % ST], (t / ST) & 1)) break;
   } else {
     // ---- softmax ---------------------------------------------------------
     regs_up<kSoftRegs>();
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // this thread's row of a piece
     struct Mine {
       bool in, present;  // has a row; the row tile has
+      bool none;         // the row sees none of the piece's keys
       int seen;
       long at, out_at;   // among the results; offset of its output
     };
@@ -400,13 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int i = p.row0 + x * kRows + quarter * 32 + lane;
       m.present = x == 0 || (tile_rows > kRows && p.row0 + kRows < p.rows);
       m.in = m.present && i < p.rows;
-      m.seen = p.k1;
+      m.none = false;
+      m.seen = p.k1;  // a row that sees nothing is let go along, and dropped at the end
       m.at = 0;
       m.out_at = 0;
       long q_at = -1;
       if (m.in) {
         const PaRow r = row_of(a, p, i);
-        m.seen = min(visible(a, p.seq < 0, r), p.k1);
+        const int seen = visible(a, p.seq < 0, r);
+        m.none = seen <= p.k0;
+        if (!m.none) m.seen = min(seen, p.k1);
         m.at = r.token * a.hq + r.h;
         m.out_at = r.token * a.ldo + static_cast<long>(r.h) * HD;
         q_at = r.token * a.ldq + static_cast<long>(r.h) * HD;
@@ -452,32 +457,75 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           const int j0 = w.k0 + j * kKeys;
           if (!wait(&s_full[x], c & 1)) break;
           const bool part = j0 + kKeys > least;  // some row stops in this tile
-          uint32_t v[4][32];  // this row's scores
+          // Scores go to p = 2^(s - ref) without their maximum being looked
+          // for. Only at a piece's first tile (next loop) and where a row's sum
+          // passes 2^15 is the reference raised; in the latter case O is
+          // rescaled and p taken again from the scores, still in registers.
+          if (j == 0 || part) {
+            // keys that a row does not see get their scores out of the way
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int cc = 0; cc < 8; ++cc) {
+              uint32_t u[16];
+              tmem_ld16(tS + cc * 16, u);
+              tmem_wait_ld();
+              const int limit = seen - j0 - cc * 16;
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, v[cc]);
-          tmem_wait_ld();
-          if (part) {
+              for (int t = 0; t < 16; ++t) {
+                if (t >= limit) u[t] = __float_as_uint(-INFINITY);
+                mx = fmaxf(mx, __uint_as_float(u[t]));
+              }
+              if (part) tmem_st16(tS + cc * 16, u);
+            }
+            if (part) tmem_wait_st();
+            if (j == 0) ref = mx * sl;
+          }
+          uint32_t v[4][32];
+          const float2 sl2 = make_float2(sl, sl);
+          float2 sum[2];
+          const auto exps = [&](int cc) {
+            const float sub = ref == -INFINITY ? 0.f : ref;
+            const float2 sub2 = make_float2(-sub, -sub);
+            uint32_t pk[16];
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+              const float2 y = __ffma2_rn(
+                  make_float2(__uint_as_float(v[cc][2 * t]), __uint_as_float(v[cc][2 * t + 1])), sl2, sub2);
+              const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+              sum[t & 1] = __fadd2_rn(sum[t & 1], p);
+              pk[t] = pack_bf16x2(p.x, p.y);
+            }
+            tmem_st16(tS + cc * 16, pk);  // over scores that have been read
+          };
+          const auto total = [&] { return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y); };
+          // 32 scores at a time, the next on their way meanwhile
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
+          tmem_ld32(tS, v[0]);
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) {
+            tmem_wait_ld();
+            if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, v[cc + 1]);
+            exps(cc);
+          }
+          float tile_l = total();
+          // A NaN is left as it is. A row without a reference sees no key so
+          // far, and so none later either.
+          if (__builtin_expect(__any_sync(0xffffffffu, tile_l > 32768.f), 0)) {
+            float m[2] = {ref, -INFINITY};
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
-              for (int t = 0; t < 32; ++t)
-                if (j0 + cc * 32 + t >= seen) v[cc][t] = __float_as_uint(-INFINITY);
-          }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int t = 0; t < 32; ++t)
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) m4[cc] = fmaxf(m4[cc], __uint_as_float(v[cc][t]));
-          float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          mx *= sl;
-          if (__any_sync(0xffffffffu, mx > ref + 8.f)) {
-            const float to = fmaxf(ref, mx);
-            const float f = to == -INFINITY ? 1.f : ex2_approx(ref - to);
-            ref = to;
+              for (int t = 0; t < 32; t += 2) {
+                m[0] = fmaxf(m[0], __uint_as_float(v[cc][t]) * sl);
+                m[1] = fmaxf(m[1], __uint_as_float(v[cc][t + 1]) * sl);
+              }
+            const float mx = fmaxf(m[0], m[1]);
+            const float f = mx == -INFINITY ? 1.f : ex2_approx(ref - mx);
+            ref = mx;
             l *= f;
             if (j > 0) {
               if (!wait(&o_full[x], (c - 1) & 1)) break;
-#pragma unroll
+#pragma unroll 1
               for (int cc = 0; cc < HD / 16; ++cc) {
                 uint32_t u[16];
                 tmem_ld16(tO + cc * 16, u);
@@ -486,32 +534,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 for (int t = 0; t < 16; ++t) u[t] = __float_as_uint(__uint_as_float(u[t]) * f);
                 tmem_st16(tO + cc * 16, u);
               }
-              tmem_wait_st();
             }
-          }
-          const float sub = ref == -INFINITY ? 0.f : ref;
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float2 sl2 = make_float2(sl, sl), sub2 = make_float2(-sub, -sub);
+            sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int t = 0; t < 32; t += 2) {
-              const float2 y =
-                  __ffma2_rn(make_float2(__uint_as_float(v[cc][t]), __uint_as_float(v[cc][t + 1])), sl2, sub2);
-              const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-              sum[(t / 2) & 1] = __fadd2_rn(sum[(t / 2) & 1], p);
-              pk[t / 2] = pack_bf16x2(p.x, p.y);
-            }
-            tmem_st16(tS + cc * 16, pk);
+            for (int cc = 0; cc < 4; ++cc) exps(cc);
+            tile_l = total();
           }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          l += tile_l;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[x]);
         }
         if (!ok) break;
+      }
+      if (mine.none) {
+        ref = -INFINITY;
+        l = 0.f;
       }
       more = pieces.next(a, next_w);
       if (more) next_mine = row_in(next_w);
@@ -538,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           their_at[k] = __shfl_sync(0xffffffffu, row_at, 8 * k + lane / 4);
           their_scale[k] = __shfl_sync(0xffffffffu, scale, 8 * k + lane / 4);
         }
-#pragma unroll
+#pragma unroll 1
         for (int cc = 0; cc < HD / 16; ++cc) {
           uint32_t v[16];
           tmem_ld16(tO + cc * 16, v);
