@@ -407,7 +407,7 @@ size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
 }  // namespace
 
 int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
-int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_items, cudaStream_t s);
+int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
 int attn_tc(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
 
 size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {

@@ -155,7 +155,7 @@ struct Rows {
   // 16 keys, number key0 of the segment on, in rows r0 .. of the tiles sk, sv.
   __device__ __forceinline__ void take(uint32_t sk, uint32_t sv, int r0, int key0, float sl) {
     const int lane = threadIdx.x % 32, t4 = lane % 4;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float s[2][4] = {};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       // matrices: keys 0-7 and 8-15, each at head_dim 0-7 and 8-15 of the step
@@ -383,10 +383,11 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(P
 
 // ---- one warp a piece: at most 16 rows -------------------------------------
 // A block is one warp with a ring of its own, 16 keys a stage, so blocks never
-// wait for one another and as many as shared memory holds (7 with 128 values a
-// head) keep the SM's copies in flight. A block takes a run of the prefix, or
-// own pieces blockIdx, blockIdx + blocks, ..; the ring runs on into the next
-// piece, whose first copies are in flight while this one ends.
+// wait for one another and as many as registers and shared memory hold (9 with
+// 128 values a head) keep the SM's copies in flight. A block takes a run of the
+// prefix or one own piece. (As many blocks as are resident, each taking every
+// so-manyth own piece, left SMs idle a quarter of the time: 512 sequences of up
+// to 256 keys took 72 us, a block each 62.)
 template <int HD>
 struct WarpShared {
   __nv_bfloat16 kv[kWarpStages][2][16 * HD];
@@ -395,25 +396,21 @@ struct WarpShared {
 
 struct WarpWork {
   PaRun run;
-  int own, step, count;  // own pieces left: own, own + step, ..
-  bool prefix;
-  __device__ __forceinline__ WarpWork(const PaArgs& a, int prefix_ctas, int own_items)
-      : run(a.prefix, a.hkv, blockIdx.x),
-        own(static_cast<int>(blockIdx.x) - prefix_ctas),
-        step(static_cast<int>(gridDim.x) - prefix_ctas),
-        count(own_items),
-        prefix(static_cast<int>(blockIdx.x) < prefix_ctas) {}
+  int own;  // the own piece, or -1
+  __device__ __forceinline__ WarpWork(const PaArgs& a, int prefix_ctas)
+      : run(a.prefix, a.hkv, blockIdx.x), own(static_cast<int>(blockIdx.x) - prefix_ctas) {
+    if (own >= 0) run.left = 0;
+  }
   __device__ __forceinline__ bool next(const PaArgs& a, PaPiece& w) {
-    if (prefix) return run.next(a, blockIdx.x, w);
-    if (own >= count) return false;
+    if (own < 0) return run.next(a, blockIdx.x, w);
     w = own_piece(a, own);
-    own += min(step, count - own);
+    own = -1;
     return true;
   }
 };
 
 template <int HD>
-__global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas, int own_items) {
+__global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   WarpShared<HD>& sh = *reinterpret_cast<WarpShared<HD>*>(smem_raw);
   using bf = __nv_bfloat16;
@@ -424,7 +421,7 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
   pdl_trigger();
 
   // the copies' place in the work, ahead of the products'
-  WarpWork ahead(a, prefix_ctas, own_items);
+  WarpWork ahead(a, prefix_ctas);
   PaPiece lw;
   lw.k1 = 0;
   int lj = 0;
@@ -460,7 +457,7 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) issue(s);
 
-  WarpWork work(a, prefix_ctas, own_items);
+  WarpWork work(a, prefix_ctas);
   PaPiece w;
   int stage = 0;
   while (work.next(a, w)) {
@@ -521,7 +518,7 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
 }
 
 template <int HD>
-int launch_warp(const PaArgs& a, int prefix_ctas, int own_items, cudaStream_t s) {
+int launch_warp(const PaArgs& a, int prefix_ctas, int own_ctas, cudaStream_t s) {
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(attn_warp_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -529,9 +526,8 @@ int launch_warp(const PaArgs& a, int prefix_ctas, int own_items, cudaStream_t s)
       return SB_OPERR_LAUNCH;
     attr = true;
   }
-  const int own_ctas = std::min(own_items, std::max(1, warp_blocks_per_sm(HD) * num_sms_cached() - prefix_ctas));
-  return launch_pdl(attn_warp_kernel<HD>, dim3(static_cast<unsigned>(prefix_ctas + own_ctas)), dim3(32),
-                    sizeof(WarpShared<HD>), s, a, prefix_ctas, own_items) == cudaSuccess
+  return launch_pdl(attn_warp_kernel<HD>, dim3(static_cast<unsigned>(prefix_ctas) + own_ctas), dim3(32),
+                    sizeof(WarpShared<HD>), s, a, prefix_ctas) == cudaSuccess
              ? 0
              : SB_OPERR_LAUNCH;
 }
@@ -559,10 +555,10 @@ int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_
   return launch<128>(a, prefix_ctas, own_ctas, s);
 }
 
-int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_items, cudaStream_t s) {
-  if (hd == 32) return launch_warp<32>(a, prefix_ctas, own_items, s);
-  if (hd == 64) return launch_warp<64>(a, prefix_ctas, own_items, s);
-  return launch_warp<128>(a, prefix_ctas, own_items, s);
+int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s) {
+  if (hd == 32) return launch_warp<32>(a, prefix_ctas, own_ctas, s);
+  if (hd == 64) return launch_warp<64>(a, prefix_ctas, own_ctas, s);
+  return launch_warp<128>(a, prefix_ctas, own_ctas, s);
 }
 
 }  // namespace sb
