@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
     const long row = token * a.group.d + (h - head * static_cast<int>(a.group.d));
     n_prefix = a.prefix.parts_of(head * a.prefix.row_tiles + static_cast<int>(row / a.prefix.tile_rows));
   }
-  const int parts = n_prefix + a.own.splits;
+  const int parts = n_prefix + a.own.parts;
   const auto slot = [&](int p) { return (p < n_prefix ? p : a.prefix.parts + p - n_prefix) * rows + at; };
   float m = -INFINITY, l = 0.f, o[C];
 #pragma unroll
@@ -305,7 +305,7 @@ struct Plan {
   PaOwn own = {};
   Kernel prefix_kernel, own_kernel;
   int own_ctas = 0;
-  long parts() const { return prefix.parts + own.splits; }
+  long parts() const { return prefix.parts + own.parts; }
 };
 
 long ceil_div(long a, long b) { return (a + b - 1) / b; }
@@ -313,18 +313,23 @@ long ceil_div(long a, long b) { return (a + b - 1) / b; }
 bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long G = d.h_q / d.cache.n_heads, hkv = d.cache.n_heads;
   const long prefix_rows = static_cast<long>(d.b) * d.tq * G, own_rows = d.tq * G;
-  const auto choose = [&](long rows) {
+  // tcgen05 tiles for more than 64 rows; from 17 rows on where every SM gets
+  // some 128-key tiles to spread a block's start and end over (8 x 4 rows
+  // behind 131072 keys: TODO us, the warp-level kernel 147; behind TODO).
+  const auto choose = [&](long rows, long items, long keys) {
     if (d.cache.elem == SB_ELEM_F32) return kSimt;
     if (rows <= 16) return kWarp;
-    return rows > 64 && tiled_rows(d.cache, 128) ? kTc : kMma;
+    if (!tiled_rows(d.cache, 128)) return kMma;
+    return rows > 64 || items * (keys / 128) >= 4L * num_sms_cached() ? kTc : kMma;
   };
   const auto rows_of = [](Kernel k, long rows) {
     if (k == kTc) return rows > 128 ? 256 : 128;
     return k == kSimt || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
   };
   const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : (k == kWarp ? 16 : kKeys)); };
-  p.prefix_kernel = choose(prefix_rows);
-  p.own_kernel = choose(own_rows);
+  const long own_capacity = static_cast<long>(d.max_pages) * d.cache.page_rows;
+  p.prefix_kernel = choose(prefix_rows, hkv, d.prefix_len);
+  p.own_kernel = choose(own_rows, d.b * hkv, own_capacity);
   p.prefix.tile_rows = rows_of(p.prefix_kernel, prefix_rows);
   p.own.tile_rows = rows_of(p.own_kernel, own_rows);
   p.prefix.tile_keys = keys_of(p.prefix_kernel);
@@ -332,7 +337,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   p.prefix.row_tiles = static_cast<int>(ceil_div(prefix_rows, p.prefix.tile_rows));
   p.own.row_tiles = static_cast<int>(ceil_div(own_rows, p.own.tile_rows));
   p.prefix.tiles = static_cast<int>(ceil_div(d.prefix_len, p.prefix.tile_keys));
-  const long own_tiles = ceil_div(static_cast<long>(d.max_pages) * d.cache.page_rows, p.own.tile_keys);
+  const long own_tiles = ceil_div(own_capacity, p.own.tile_keys);
   const long prefix_work = hkv * p.prefix.row_tiles * p.prefix.tiles;
   const long own_items = d.b * hkv * p.own.row_tiles, own_work = own_items * own_tiles;
   // Key tiles that a block takes: at least 2, and enough that all blocks of a
@@ -347,10 +352,16 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   if (prefix_work + prefix_quota > 0x7fffffffL) return false;  // counted in 32 bits
   p.prefix.per_cta = static_cast<int>(prefix_quota);
   p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, prefix_quota));
+  // a block of the tcgen05 kernel with one row tile deals its key tiles out to
+  // both of its softmax groups
+  p.prefix.slots = p.prefix_kernel == kTc && p.prefix.tile_rows == 128 ? 2 : 1;
+  p.own.slots = p.own_kernel == kTc && p.own.tile_rows == 128 ? 2 : 1;
   p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / prefix_quota + 2) : 0;
   if (p.prefix.tiles > 0 && prefix_quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
+  p.prefix.parts *= p.prefix.slots;
   p.own.splits = static_cast<int>(std::min(256L, ceil_div(own_tiles, own_quota)));
-  if (p.parts() == 0) p.own.splits = 1;  // no keys at all: one empty part
+  if (p.prefix.parts + p.own.splits == 0) p.own.splits = 1;  // no keys at all: an empty part
+  p.own.parts = p.own.splits * p.own.slots;
   const long own_ctas = own_items * p.own.splits;
   if (own_ctas + p.prefix.ctas > 0x7fffffffL) return false;
   p.own_ctas = static_cast<int>(own_ctas);
@@ -390,7 +401,7 @@ int simt(const PaArgs& a, int own_ctas, cudaStream_t s) {
 template <typename T, int HD>
 int join(const PaArgs& a, cudaStream_t s) {
   const long rows = static_cast<long>(a.b) * a.tq * a.hq;
-  const bool wide = a.prefix.parts + a.own.splits > 8;
+  const bool wide = a.prefix.parts + a.own.parts > 8;
   const dim3 grid(static_cast<unsigned>(wide ? rows : (rows + 7) / 8));
   return launch_pdl(wide ? attn_join_kernel<T, HD, 8> : attn_join_kernel<T, HD, 1>, grid, dim3(256), 0, s, a) ==
                  cudaSuccess

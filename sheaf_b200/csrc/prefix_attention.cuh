@@ -41,25 +41,27 @@ struct FastDiv {
 
 // How the prefix's work is cut: items (key head, tile of rows) of `tiles` key
 // tiles each, one after the other, in runs of `per_cta` key tiles a block,
-// whatever items a run touches. Item i leaves its part n = block - first(i).
+// whatever items a run touches. Block b leaves parts (b - first(i)) * slots ..
+// of item i, one for each of its slots (rows whose keys it splits once more).
 struct PaPrefix {
   int row_tiles;  // of a key head
   int tile_rows, tile_keys;
   int tiles, per_cta, ctas;
+  int slots;
   int parts;      // most parts an item has
   // (all key tiles together stay below 2^31)
   __host__ __device__ __forceinline__ int first(int item) const {
     return static_cast<uint32_t>(item * tiles) / static_cast<uint32_t>(per_cta);
   }
   __host__ __device__ __forceinline__ int parts_of(int item) const {
-    return static_cast<int>(static_cast<uint32_t>((item + 1) * tiles - 1) / static_cast<uint32_t>(per_cta)) -
-           first(item) + 1;
+    return slots * (static_cast<int>(static_cast<uint32_t>((item + 1) * tiles - 1) / static_cast<uint32_t>(per_cta)) -
+                    first(item) + 1);
   }
 };
 // The sequences' own keys: items (sequence, key head, tile of rows), each cut
-// evenly into `splits`, a block each.
+// evenly into `splits`, a block each, which leaves `slots` parts.
 struct PaOwn {
-  int row_tiles, tile_rows, tile_keys, splits;
+  int row_tiles, tile_rows, tile_keys, splits, slots, parts;
 };
 
 struct PaArgs {
@@ -100,7 +102,7 @@ struct PaPiece {
   int head;    // key head
   int row0;    // first of the tile's rows among the segment's
   int rows;    // the segment's rows
-  int part;    // where its partial results go
+  int part;    // where its (first slot's) partial results go
   int k0, k1;  // keys
 };
 
@@ -159,7 +161,7 @@ struct PaRun {
     w.head = static_cast<uint32_t>(item) / static_cast<uint32_t>(p.row_tiles);
     w.row0 = (item - w.head * p.row_tiles) * p.tile_rows;
     w.rows = a.b * a.seq_rows.d;
-    w.part = cta - p.first(item);
+    w.part = (cta - p.first(item)) * p.slots;
     w.k0 = tile * p.tile_keys;
     w.k1 = min((tile + n) * p.tile_keys, a.prefix_len);
     left -= n;
@@ -182,7 +184,7 @@ __device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
   const int split = i - w.seq * o.splits;
   w.row0 = tile * o.tile_rows;
   w.rows = a.seq_rows.d;
-  w.part = a.prefix.parts + split;
+  w.part = a.prefix.parts + split * o.slots;
   // keys that the tile's last row sees
   const int n = max(seq_len(a, w.seq), 0);
   const int last = a.group(min(w.row0 + o.tile_rows, w.rows) - 1);  // its query

@@ -20,6 +20,8 @@
 //   warp 11   looks through the tiles of V in which a row stops (below).
 // The softmax warps gather their rows of Q, those of the next piece while the
 // last products of this one run.
+// With at most 128 rows the two softmax groups take the same rows and the key
+// tiles in turn, each with an output of its own (two parts).
 // TMEM: S_0, S_1 (128 columns each), O_0, O_1 (HD each).
 #include <algorithm>
 
@@ -334,10 +336,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         umma_commit(&s_full[x]);
       }
     };
+    const auto product = [&](int x, bool more) {  // O_x (+)= P_x V
+      if (one) {
+        const uint64_t v = dv + vst * kStep;
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          umma_f16_tmem_a(tmem + L::kTmemO + x * HD, tmem + x * 128 + kk * 8, v + ((kk * 2048) >> 4), idO,
+                          (more || kk > 0) ? 1u : 0u);
+        umma_commit(&o_full[x]);
+      }
+    };
+    const auto next_k = [&] {  // the products issued are the last to read this stage
+      if (one) umma_commit(&k_empty[kst]);
+      kst = kst + 1 == ST ? 0 : kst + 1;
+      kph ^= kst == 0;
+    };
+    const auto next_v = [&] {
+      if (one) umma_commit(&v_empty[vst]);
+      vst = vst + 1 == ST ? 0 : vst + 1;
+      vph ^= vst == 0;
+    };
     while (ok && pieces.next(a, w)) {
       if (w.k1 <= w.k0) continue;
       const int n = (w.k1 - w.k0 + kKeys - 1) / kKeys;
-      const int tiles = (tile_rows > kRows && w.row0 + kRows < w.rows) ? 2 : 1;
+      if (tile_rows == kRows) {
+        // one row tile: key tile j for softmax group j % 2
+        for (int j = 0; j < min(n, 2); ++j) {
+          if (!wait(&k_full[kst], kph) || !wait(&q_full[j], begun[j]++ & 1)) break;
+          scores(j);
+          next_k();
+        }
+        if (!ok) break;
+        for (int j = 0; j < n; ++j, ++c) {
+          const int x = j & 1;
+          if (!wait(&v_full[vst], vph) || !wait(&p_full[x], done[x]++ & 1)) break;
+          product(x, j > 1);
+          next_v();
+          if (j + 2 < n) {
+            if (!wait(&k_full[kst], kph)) break;
+            scores(x);
+            next_k();
+          }
+        }
+        continue;
+      }
+      const int tiles = w.row0 + kRows < w.rows ? 2 : 1;
       if (!wait(&k_full[kst], kph)) break;
       for (int x = 0; x < tiles; ++x) {
         if (!wait(&q_full[x], begun[x]++ & 1)) break;
@@ -345,29 +388,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       if (!ok) break;
       for (int j = 0; j < n; ++j, ++c) {
-        if (one) umma_commit(&k_empty[kst]);
-        kst = kst + 1 == ST ? 0 : kst + 1;
-        kph ^= kst == 0;
+        next_k();
         if (!wait(&v_full[vst], vph)) break;
-        const uint64_t v = dv + vst * kStep;
         for (int x = 0; x < tiles; ++x) {
           if (!wait(&p_full[x], done[x]++ & 1)) break;
-          if (one) {
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              umma_f16_tmem_a(tmem + L::kTmemO + x * HD, tmem + x * 128 + kk * 8, v + ((kk * 2048) >> 4), idO,
-                              (j > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&o_full[x]);
-          }
+          product(x, j > 0);
           if (j + 1 < n) {
             if (x == 0 && !wait(&k_full[kst], kph)) break;
             scores(x);
           }
         }
         if (!ok) break;
-        if (one) umma_commit(&v_empty[vst]);
-        vst = vst + 1 == ST ? 0 : vst + 1;
-        vph ^= vst == 0;
+        next_v();
       }
     }
     // no commit may arrive on this block's barriers after it has exited
@@ -378,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // ---- softmax ---------------------------------------------------------
     regs_up<kSoftRegs>();
     const int x = warp / 4, quarter = warp % 4;
+    const bool deal = tile_rows == kRows;  // key tiles go to the two groups in turn
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lanes + x * 128, tO = tmem + lanes + L::kTmemO + x * HD;
     const float sl = a.scale * 1.4426950408889634f;
@@ -392,16 +425,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     };
     // this thread's row of a piece
     struct Mine {
-      bool in, present;  // has a row; the row tile has
+      bool in;           // has a row
       bool none;         // the row sees none of the piece's keys
+      int tiles;         // key tiles that this group takes
       int seen;
       long at, out_at;   // among the results; offset of its output
     };
     const auto row_in = [&](const PaPiece& p) {
       Mine m;
-      const int i = p.row0 + x * kRows + quarter * 32 + lane;
-      m.present = x == 0 || (tile_rows > kRows && p.row0 + kRows < p.rows);
-      m.in = m.present && i < p.rows;
+      const int i = p.row0 + (deal ? 0 : x * kRows) + quarter * 32 + lane;
+      m.in = i < p.rows;
+      m.tiles = (max(p.k1 - p.k0, 0) + kKeys - 1) / kKeys;
+      if (deal)
+        m.tiles = (m.tiles + 1 - x) / 2;
+      else if (x == 1 && p.row0 + kRows >= p.rows)
+        m.tiles = 0;
       m.none = false;
       m.seen = p.k1;  // a row that sees nothing is let go along, and dropped at the end
       m.at = 0;
@@ -418,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       // this warp's rows of Q; rows past the segment's end are zero. The
       // row tile's last scores are done: Q is free.
-      if (m.present && p.k1 > p.k0) {
+      if (m.tiles > 0) {
         constexpr int CH = HD / 8, RPI = 32 / CH;  // rows an instruction
 #pragma unroll
         for (int n = 0; n < 32 / RPI; ++n) {
@@ -431,30 +469,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       cp_async_commit();
       return m;
     };
-    const auto announce_q = [&](const Mine& m, const PaPiece& p) {
+    const auto announce_q = [&](const Mine& m) {
       cp_async_wait<0>();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && m.present && p.k1 > p.k0) mbar_arrive(&q_full[x]);
+      if (lane == 0 && m.tiles > 0) mbar_arrive(&q_full[x]);
     };
     PaPiece next_w;
     bool more = pieces.next(a, next_w);
     Mine next_mine = {};
     if (more) {
       next_mine = row_in(next_w);
-      announce_q(next_mine, next_w);
+      announce_q(next_mine);
     }
     while (ok && more) {
       w = next_w;
       const Mine mine = next_mine;
-      const bool work = w.k1 > w.k0, present = mine.present;
-      const int n = work ? (w.k1 - w.k0 + kKeys - 1) / kKeys : 0;
       const int seen = mine.seen;
       const int least = __reduce_min_sync(0xffffffffu, seen);
       float ref = -INFINITY, l = 0.f;
-      if (present) {
-        for (int j = 0; j < n; ++j, ++c) {
-          const int j0 = w.k0 + j * kKeys;
+      for (int j = 0; j < mine.tiles; ++j, ++c) {
+          const int j0 = w.k0 + (deal ? 2 * j + x : j) * kKeys;
           if (!wait(&s_full[x], c & 1)) break;
           const bool part = j0 + kKeys > least;  // some row stops in this tile
           // Scores go to p = 2^(s - ref) without their maximum being looked
@@ -545,18 +580,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[x]);
-        }
-        if (!ok) break;
       }
+      if (!ok) break;
       if (mine.none) {
         ref = -INFINITY;
         l = 0.f;
       }
       more = pieces.next(a, next_w);
       if (more) next_mine = row_in(next_w);
-      if (present && n > 0 && !wait(&o_full[x], (c - 1) & 1)) break;
+      if (mine.tiles > 0 && !wait(&o_full[x], (c - 1) & 1)) break;
       const float nat = ref * 0.6931471805599453f;  // natural units outside
-      const long part_at = static_cast<long>(w.part) * a.b * a.tq * a.hq + mine.at;
+      const long part_at = static_cast<long>(w.part + (deal ? x : 0)) * a.b * a.tq * a.hq + mine.at;
       if (mine.in) {
         if (a.direct) {
           if (a.lse) a.lse[mine.at] = nat + logf(l);
@@ -565,8 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
       }
       // rows leave through shared memory, 64 bytes of 8 rows a store
-      if (present && (n > 0 || a.direct)) {
-        const bool some = n > 0 && *reinterpret_cast<volatile const int*>(sm + L::kFound) == piece + 1;
+      if (mine.tiles > 0 || a.direct) {
+        const bool some = mine.tiles > 0 && *reinterpret_cast<volatile const int*>(sm + L::kFound) == piece + 1;
         const int* bad = reinterpret_cast<const int*>(sm + L::kBad);
         const long row_at = !mine.in || (!a.direct && l == 0.f) ? -1 : (a.direct ? mine.out_at : part_at * HD);
         const float scale = a.direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
@@ -611,8 +645,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
       }
       tc_fence_before();  // O is read before the next piece's P is announced
-      if (more) announce_q(next_mine, next_w);
-      if (work) {
+      if (more) announce_q(next_mine);
+      if (w.k1 > w.k0) {
         ++piece;
         __syncwarp();
         if (lane == 0) reinterpret_cast<volatile int*>(sm + L::kDone)[warp] = piece;
