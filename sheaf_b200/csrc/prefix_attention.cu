@@ -320,7 +320,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
     if (d.cache.elem == SB_ELEM_F32) return kSimt;
     if (rows <= 16) return kWarp;
     if (!tiled_rows(d.cache, 128)) return kMma;
-    return rows > 64 || items * (keys / 128) >= 4L * num_sms_cached() ? kTc : kMma;
+    return rows > 64 || items * (keys / 128) >= 100L ? kTc : kMma;
   };
   const auto rows_of = [](Kernel k, long rows) {
     if (k == kTc) return rows > 128 ? 256 : 128;
