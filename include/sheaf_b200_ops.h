@@ -247,7 +247,7 @@ SB_API int sb_op_prefix_attention(const sb_kv_cache* cache, const void* q, int64
                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* Scores rows of logits [rows, v] (row stride ld, any alignment) at a
- * temperature > 0, with z = logits / temperature:
+ * temperature in [1e-6, 1e6], with z = logits / temperature:
  *   logp [rows]    = z[t] - lse for the row's given token t (f32 class id as
  *                    in sb_op_cross_entropy: one that is not exactly an
  *                    integer in [0, v) gives 0)

@@ -342,7 +342,7 @@ int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, int32_t 
                          void* top_logp, void* stream) {
   if (!float_elem(elem) || rows < 0 || v <= 0 || v > (1 << 30) || !fits(ld) || ld < v || k < 0 || k > SB_LOGPROBS_MAX_TOP || k > v)
     return SB_OPERR_ARGS;
-  if (!(temperature > 0.f) || !std::isfinite(temperature)) return SB_OPERR_ARGS;
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) return SB_OPERR_ARGS;
   if (rows == 0) return 0;
   if (!logits || !on_values(logits, elem) || (logp && !targets)) return SB_OPERR_ARGS;
   sb::LogprobsDesc d;
@@ -366,7 +366,7 @@ int sb_op_token_logprobs_bwd(uint32_t elem, const void* logits, int64_t ld, int3
                              const void* targets, float temperature, const void* lse, const void* entropy,
                              const void* dlogp, const void* dentropy, void* dlogits, int64_t ldd, void* stream) {
   if (!float_elem(elem) || rows < 0 || v <= 0 || v > (1 << 30) || !fits(ld) || !fits(ldd) || ld < v || ldd < v) return SB_OPERR_ARGS;
-  if (!(temperature > 0.f) || !std::isfinite(temperature)) return SB_OPERR_ARGS;
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) return SB_OPERR_ARGS;
   if (rows == 0) return 0;
   if (!logits || !dlogits || !lse || !on_values(logits, elem) || !on_values(dlogits, elem)) return SB_OPERR_ARGS;
   if ((dlogp && !targets) || (dentropy && !entropy)) return SB_OPERR_ARGS;

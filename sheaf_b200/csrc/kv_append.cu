@@ -41,7 +41,9 @@ struct AppendArgs {
   T* k;
   T* v;
   long page_stride, row_stride, head_stride;
-  int n_pages, page_rows, hkv, hd;
+  int n_pages, hkv, hd;
+  FastDiv page_rows;
+  FastDiv units, per_token;  // units of a head; threads of a token
   const T* qkv;
   long ld;
   int n, hq;
@@ -62,14 +64,13 @@ struct AppendArgs {
 template <typename T, int VEC, int MODE, int HPT>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs<T> a) {
   using P = Pack<T, VEC>;
-  const int units = a.hd / (2 * VEC);               // units of a head
   const int heads = a.hq + 2 * a.hkv;
-  const int groups = (heads + HPT - 1) / HPT;
-  const long idx = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long token = idx / (units * groups);
-  if (token >= a.n) return;
-  const int rest = static_cast<int>(idx - token * (units * groups));
-  const int h0 = rest / units * HPT, u = rest % units;
+  const uint32_t idx = blockIdx.x * blockDim.x + threadIdx.x;
+  const uint32_t t = a.per_token(idx);
+  if (t >= static_cast<uint32_t>(a.n)) return;
+  const long token = t;
+  const uint32_t rest = idx - t * a.per_token.d, group = a.units(rest);
+  const int h0 = group * HPT, u = rest - group * a.units.d;
 
   // element offsets of the unit's two vectors within a head
   const int half = a.rot / 2;
@@ -97,15 +98,15 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs<T> a) {
   const int s = a.seq[token], p = a.pos[token];
   bool live = s >= 0;  // a negative sequence marks a padding token
   if (live && (s >= a.n_seqs || p < a.base || (MODE != kRotNone && p >= a.n_pos) ||
-               (p - a.base) / a.page_rows >= a.max_pages)) {
+               static_cast<int>(a.page_rows(p - a.base)) >= a.max_pages)) {
     live = false;
     if (a.err) atomicExch(a.err, kErrIndex);
   }
   long row = -1;  // element offset of the token's row in the cache
   if (live) {
-    const int own = p - a.base, page = a.pages[static_cast<long>(s) * a.max_pages + own / a.page_rows];
+    const int own = p - a.base, nth = a.page_rows(own), page = a.pages[static_cast<long>(s) * a.max_pages + nth];
     if (page >= 0 && page < a.n_pages)
-      row = page * a.page_stride + static_cast<long>(own % a.page_rows) * a.row_stride;
+      row = page * a.page_stride + static_cast<long>(own - nth * static_cast<int>(a.page_rows.d)) * a.row_stride;
     else if (a.err)
       atomicExch(a.err, kErrIndex);
   }
@@ -168,12 +169,22 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs<T> a) {
 }
 
 template <typename T, int VEC, int MODE, int HPT>
-int launch(const AppendArgs<T>& a, cudaStream_t s) {
-  const long groups = (a.hq + 2 * a.hkv + HPT - 1) / HPT;
-  const long threads = a.n * groups * (a.hd / (2 * VEC));
-  const long blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffL) return SB_OPERR_ARGS;
-  kv_append_kernel<T, VEC, MODE, HPT><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+int launch(AppendArgs<T> a, cudaStream_t s) {
+  const int groups = (a.hq + 2 * a.hkv + HPT - 1) / HPT, units = a.hd / (2 * VEC);
+  a.units = FastDiv::of(units);
+  a.per_token = FastDiv::of(groups * units);
+  // threads are counted in 31 bits: more tokens than that take several launches
+  const int most = std::max(1, 0x7fff0000 / (groups * units)), n = a.n;
+  for (int at = 0; at < n; at += std::min(most, n - at)) {
+    AppendArgs<T> part = a;
+    part.n = std::min(most, n - at);
+    part.qkv += at * a.ld;
+    part.q_out += a.hq ? at * a.ldq : 0;
+    part.seq += at;
+    part.pos += at;
+    const unsigned blocks = (static_cast<unsigned>(part.n) * (groups * units) + 255) / 256;
+    kv_append_kernel<T, VEC, MODE, HPT><<<blocks, 256, 0, s>>>(part);
+  }
   return cudaPeekAtLastError() == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
 }
 
@@ -193,7 +204,7 @@ int append_t(const AppendDesc& d, cudaStream_t s, int* err) {
   a.row_stride = d.cache.row_stride;
   a.head_stride = d.cache.head_stride;
   a.n_pages = d.cache.n_pages;
-  a.page_rows = d.cache.page_rows;
+  a.page_rows = FastDiv::of(d.cache.page_rows);
   a.hkv = d.cache.n_heads;
   a.hd = d.cache.head_dim;
   a.qkv = static_cast<const T*>(d.qkv);
@@ -222,7 +233,7 @@ int append_t(const AppendDesc& d, cudaStream_t s, int* err) {
   // whole units of pairs, and angle rows that start on 16 bytes
   if (a.rot) vec = vec && a.rot % (2 * VEC) == 0 && a.rot % 8 == 0 && table(d.cos) && table(d.sin);
   if (!vec) return by_mode<T, 1, 1>(a, d.rotary, s);
-  return by_mode<T, VEC, 4>(a, d.rotary, s);
+  return by_mode<T, VEC, 2>(a, d.rotary, s);
 }
 
 }  // namespace

@@ -14,6 +14,25 @@ namespace sb {
 // kernel skips the access and records this (sb_op_device_error).
 constexpr int kErrIndex = 2;
 
+// Division of a non-negative 31-bit number by a fixed d >= 1: n / d =
+// (n * mul) >> 32 >> shift with mul = floor(2^(32 + shift) / d) + 1, 2^shift
+// the power of two just below d (exact for n < 2^31; Granlund and Montgomery,
+// PLDI 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  static FastDiv of(uint32_t d) {
+    FastDiv f{d, 0, 0};
+    if (d == 1) return f;
+    while ((2u << f.shift) < d) ++f.shift;
+    f.mul = static_cast<uint32_t>(((1ull << (32 + f.shift)) / d) + 1);
+    return f;
+  }
+  __host__ __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    if (d == 1) return n;
+    return static_cast<uint32_t>((static_cast<unsigned long long>(n) * mul) >> 32) >> shift;
+  }
+};
+
 struct AppendDesc {
   sb_kv_cache cache;
   const void* qkv;
