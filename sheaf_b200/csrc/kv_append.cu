@@ -62,7 +62,7 @@ struct AppendArgs {
 };
 
 template <typename T, int VEC, int MODE, int HPT>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs<T> a) {
+__global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
   using P = Pack<T, VEC>;
   const int heads = a.hq + 2 * a.hkv;
   const uint32_t idx = blockIdx.x * blockDim.x + threadIdx.x;

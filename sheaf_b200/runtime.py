@@ -220,12 +220,97 @@ class Session:
             raise SheafB200Error(3, f"get_batch failed ({rc})")
         return x, y
 
+    # -- cached generation and scoring -----------------------------------------
+    def _op(self, what: str, rc: int) -> None:
+        if rc:
+            raise SheafB200Error(3, f"{what} failed ({rc})")
+
+    def kv_cache(self, n_pages: int, page_rows: int, n_heads: int, head_dim: int, elem: int = ELEM_BF16) -> "KvPages":
+        """One layer's paged keys and values, [n_pages, page_rows, n_heads, head_dim] each."""
+        return KvPages(self, n_pages, page_rows, n_heads, head_dim, elem)
+
+    def kv_append(self, cache: "KvPages", qkv: "Buffer", seq: "Buffer", pos: "Buffer", pages: "Buffer", base: int = 0,
+                  rotary: int = 0, cos: "Buffer | None" = None, sin: "Buffer | None" = None) -> "Buffer":
+        """Appends the keys and values of qkv [n, (h_q + 2 h_kv) hd] at positions pos [n] of sequences seq [n] (pages
+        [n_seqs, max_pages] from position base on; i32) and returns the queries [n, h_q hd], rotated as the keys are
+        (rotary 1: halves, 2: pairs; cos, sin f32 [n_pos, rot_dim / 2])."""
+        n, width = qkv.shape
+        c = cache.desc
+        h_q = width // c.head_dim - 2 * c.n_heads
+        q = self.empty((n, h_q * c.head_dim), qkv.elem)
+        n_pos, rot = (cos.shape[0], 2 * cos.shape[1]) if rotary else (0, 0)
+        self._op("kv_append", lib().sb_op_kv_append(
+            c, qkv.device_ptr, width, n, h_q, q.device_ptr, h_q * c.head_dim, seq.device_ptr, pos.device_ptr, base,
+            pages.device_ptr, pages.shape[0], pages.shape[1], rotary, rot, cos.device_ptr if rotary else None,
+            sin.device_ptr if rotary else None, n_pos, self.stream))
+        return q
+
+    def prefix_attention(self, cache: "KvPages", q: "Buffer", lens: "Buffer", pages: "Buffer | None" = None,
+                         prefix_pages: "Buffer | None" = None, prefix_len: int = 0,
+                         scale: float | None = None) -> tuple["Buffer", "Buffer"]:
+        """Attention of q [b tq, h_q hd] (b = the entries of lens, i32) to the prefix_len keys that all sequences share
+        and each one's own lens[s] keys; returns the output and the log-sum-exp [b tq, h_q] (f32)."""
+        c = cache.desc
+        rows, width = q.shape
+        b = lens.shape[0]
+        h_q, max_pages = width // c.head_dim, pages.shape[1] if pages is not None else 0
+        out, lse = self.empty((rows, width), q.elem), self.empty((rows, h_q), ELEM_F32)
+        shape = (c, b, rows // b if b else 0, h_q, prefix_len, max_pages)
+        size = lib().sb_op_prefix_attention_workspace_size(*shape)
+        ws = self.empty(((size + 3) // 4,), ELEM_F32) if size else None
+        self._op("prefix_attention", lib().sb_op_prefix_attention(
+            c, q.device_ptr, width, out.device_ptr, width, lse.device_ptr, b, shape[2], h_q,
+            c.head_dim ** -0.5 if scale is None else scale, prefix_pages.device_ptr if prefix_pages else None, prefix_len,
+            pages.device_ptr if pages else None, max_pages, lens.device_ptr, ws.device_ptr if ws else None, size,
+            self.stream))
+        return out, lse
+
+    def token_logprobs(self, logits: "Buffer", v: int, targets: "Buffer | None" = None, temperature: float = 1.0,
+                       k: int = 0) -> dict[str, "Buffer"]:
+        """Scores the first v columns of logits [rows, ld] at a temperature: "entropy", "lse" [rows], with targets (f32
+        ids) their "logp", with k the likeliest tokens "top_ids" (i32) and "top_logp" [rows, k]."""
+        rows, ld = logits.shape
+        out = {name: self.empty((rows,), ELEM_F32) for name in ("entropy", "lse")}
+        if targets is not None:
+            out["logp"] = self.empty((rows,), ELEM_F32)
+        if k:
+            out["top_ids"], out["top_logp"] = self.empty((rows, k), ELEM_I32), self.empty((rows, k), ELEM_F32)
+        p = {name: out[name].device_ptr if name in out else None for name in
+             ("logp", "entropy", "lse", "top_ids", "top_logp")}
+        self._op("token_logprobs", lib().sb_op_token_logprobs(
+            logits.elem, logits.device_ptr, ld, rows, v, targets.device_ptr if targets is not None else None, temperature,
+            p["logp"], p["entropy"], p["lse"], k, p["top_ids"], p["top_logp"], self.stream))
+        return out
+
+    def token_logprobs_vjp(self, logits: "Buffer", v: int, scores: dict[str, "Buffer"], targets: "Buffer | None" = None,
+                           dlogp: "Buffer | None" = None, dentropy: "Buffer | None" = None,
+                           temperature: float = 1.0) -> "Buffer":
+        """Gradient [rows, ld] of sum(dlogp logp) + sum(dentropy entropy) in the logits, from token_logprobs's scores;
+        columns from v on are not written."""
+        rows, ld = logits.shape
+        dx = self.empty((rows, ld), logits.elem)
+        ptr = lambda b: b.device_ptr if b is not None else None  # noqa: E731
+        self._op("token_logprobs_vjp", lib().sb_op_token_logprobs_bwd(
+            logits.elem, logits.device_ptr, ld, rows, v, ptr(targets), temperature, scores["lse"].device_ptr,
+            scores["entropy"].device_ptr, ptr(dlogp), ptr(dentropy), dx.device_ptr, ld, self.stream))
+        return dx
+
     def call(self, qualified_name: str, inputs: Sequence["Buffer"], max_outputs: int = 1024) -> "Outputs":
         arr = (C.c_void_p * max(1, len(inputs)))(*[b._h for b in inputs])
         outs = (C.c_void_p * max_outputs)()
         n = C.c_size_t()
         _check(lib().sb_call(self._h, qualified_name.encode(), arr, len(inputs), outs, max_outputs, C.byref(n)))
         return Outputs(outs, n.value)
+
+
+class KvPages:
+    """A paged key / value cache (sb_kv_cache): its buffers and their description."""
+
+    def __init__(self, session: Session, n_pages: int, page_rows: int, n_heads: int, head_dim: int, elem: int):
+        shape = (n_pages, page_rows, n_heads, head_dim)
+        self.k, self.v = session.empty(shape, elem), session.empty(shape, elem)
+        self.desc = _lib.KvCache(self.k.device_ptr, self.v.device_ptr, page_rows * n_heads * head_dim,
+                                 n_heads * head_dim, head_dim, n_pages, page_rows, n_heads, head_dim, elem)
 
 
 # ---- leaving a data-parallel group between steps -------------------------
