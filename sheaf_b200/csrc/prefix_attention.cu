@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
   pdl_trigger();
   const int cta = blockIdx.x;
   if (cta < a.prefix.ctas) {
-    PaRun run(a.prefix, a.hkv, cta);
+    PaRun run(a.prefix, a.hkv.d, cta);
     PaPiece w;
     while (run.next(a, cta, w)) attend_piece<HD>(a, w, sh);
   } else {
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(PaArgs a) {
   if (a.prefix.ctas > 0) {
     const int head = a.group(h);
     const long row = token * a.group.d + (h - head * static_cast<int>(a.group.d));
-    n_prefix = a.prefix.parts_of(head * a.prefix.row_tiles + static_cast<int>(row / a.prefix.tile_rows));
+    n_prefix = a.prefix.parts_of(head * static_cast<int>(a.prefix.row_tiles.d) + static_cast<int>(row / a.prefix.tile_rows));
   }
   const int parts = n_prefix + a.own.parts;
   const auto slot = [&](int p) { return (p < n_prefix ? p : a.prefix.parts + p - n_prefix) * rows + at; };
@@ -334,12 +334,11 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   p.own.tile_rows = rows_of(p.own_kernel, own_rows);
   p.prefix.tile_keys = keys_of(p.prefix_kernel);
   p.own.tile_keys = keys_of(p.own_kernel);
-  p.prefix.row_tiles = static_cast<int>(ceil_div(prefix_rows, p.prefix.tile_rows));
-  p.own.row_tiles = static_cast<int>(ceil_div(own_rows, p.own.tile_rows));
-  p.prefix.tiles = static_cast<int>(ceil_div(d.prefix_len, p.prefix.tile_keys));
-  const long own_tiles = ceil_div(own_capacity, p.own.tile_keys);
-  const long prefix_work = hkv * p.prefix.row_tiles * p.prefix.tiles;
-  const long own_items = d.b * hkv * p.own.row_tiles, own_work = own_items * own_tiles;
+  const long prefix_row_tiles = ceil_div(prefix_rows, p.prefix.tile_rows);
+  const long own_row_tiles = ceil_div(own_rows, p.own.tile_rows);
+  const long prefix_tiles = ceil_div(d.prefix_len, p.prefix.tile_keys), own_tiles = ceil_div(own_capacity, p.own.tile_keys);
+  const long prefix_work = hkv * prefix_row_tiles * prefix_tiles;
+  const long own_items = d.b * hkv * own_row_tiles, own_work = own_items * own_tiles;
   // Key tiles that a block takes: at least 2, and enough that all blocks of a
   // launch are resident at once.
   const bool together = p.prefix_kernel == p.own_kernel;
@@ -350,19 +349,23 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
   const long own_quota = quota(p.own_kernel, own_work + (together ? prefix_work : 0));
   if (prefix_work + prefix_quota > 0x7fffffffL) return false;  // counted in 32 bits
-  p.prefix.per_cta = static_cast<int>(prefix_quota);
+  p.prefix.row_tiles = FastDiv::of(static_cast<uint32_t>(prefix_row_tiles));
+  p.prefix.tiles = FastDiv::of(static_cast<uint32_t>(std::max(1L, prefix_tiles)));
+  p.prefix.per_cta = FastDiv::of(static_cast<uint32_t>(prefix_quota));
   p.prefix.ctas = static_cast<int>(ceil_div(prefix_work, prefix_quota));
-  // a block of the tcgen05 kernel with one row tile deals its key tiles out to
-  // both of its softmax groups
-  p.prefix.slots = p.prefix_kernel == kTc && p.prefix.tile_rows == 128 ? 2 : 1;
-  p.own.slots = p.own_kernel == kTc && p.own.tile_rows == 128 ? 2 : 1;
-  p.prefix.parts = prefix_work ? static_cast<int>((p.prefix.tiles - 1) / prefix_quota + 2) : 0;
-  if (p.prefix.tiles > 0 && prefix_quota % p.prefix.tiles == 0) p.prefix.parts = 1;  // whole items a block
+  long splits = std::min(256L, ceil_div(own_tiles, own_quota));
+  if (prefix_work + splits == 0) splits = 1;  // no keys at all: an empty part
+  // a block of the tcgen05 kernel with one row tile deals its key tiles, where
+  // it has several, out to both of its softmax groups
+  p.prefix.slots = p.prefix_kernel == kTc && p.prefix.tile_rows == 128 && prefix_tiles > 1 ? 2 : 1;
+  p.own.slots = p.own_kernel == kTc && p.own.tile_rows == 128 && own_tiles >= 2 * splits ? 2 : 1;
+  p.prefix.parts = prefix_work ? static_cast<int>((prefix_tiles - 1) / prefix_quota + 2) : 0;
+  if (prefix_work && prefix_quota % prefix_tiles == 0) p.prefix.parts = 1;  // whole items a block
   p.prefix.parts *= p.prefix.slots;
-  p.own.splits = static_cast<int>(std::min(256L, ceil_div(own_tiles, own_quota)));
-  if (p.prefix.parts + p.own.splits == 0) p.own.splits = 1;  // no keys at all: an empty part
-  p.own.parts = p.own.splits * p.own.slots;
-  const long own_ctas = own_items * p.own.splits;
+  p.own.row_tiles = FastDiv::of(static_cast<uint32_t>(own_row_tiles));
+  p.own.splits = FastDiv::of(static_cast<uint32_t>(std::max(1L, splits)));
+  p.own.parts = static_cast<int>(splits) * p.own.slots;
+  const long own_ctas = own_items * splits;
   if (own_ctas + p.prefix.ctas > 0x7fffffffL) return false;
   p.own_ctas = static_cast<int>(own_ctas);
   return true;
@@ -373,7 +376,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
 // Tensor map over the pages of k or v: [page][row][head][head_dim], boxes of
 // 64 values of a head in box_rows rows.
 bool cache_map(void* map, const void* base, const PaArgs& a, int hd) {
-  const long dims[4] = {hd, a.hkv, static_cast<long>(a.page_rows.d), a.n_pages};
+  const long dims[4] = {hd, static_cast<long>(a.hkv.d), static_cast<long>(a.page_rows.d), a.n_pages};
   // the stride of a dimension of one is free, but the map wants a usable one
   const auto bytes = [&](long s, long count) { return count == 1 ? 16 * 16 : s * 2; };
   const long strides[3] = {bytes(a.head_stride, dims[1]), bytes(a.row_stride, dims[2]), bytes(a.page_stride, dims[3])};
@@ -438,7 +441,7 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   a.row_stride = d.cache.row_stride;
   a.head_stride = d.cache.head_stride;
   a.n_pages = d.cache.n_pages;
-  a.hkv = d.cache.n_heads;
+  a.hkv = FastDiv::of(d.cache.n_heads);
   a.page_rows = FastDiv::of(d.cache.page_rows);
   a.q = d.q;
   a.ldq = d.ldq;

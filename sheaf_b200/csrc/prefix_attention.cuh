@@ -25,32 +25,33 @@ namespace sb {
 // whatever items a run touches. Block b leaves parts (b - first(i)) * slots ..
 // of item i, one for each of its slots (rows whose keys it splits once more).
 struct PaPrefix {
-  int row_tiles;  // of a key head
+  FastDiv row_tiles;  // of a key head
   int tile_rows, tile_keys;
-  int tiles, per_cta, ctas;
+  FastDiv tiles, per_cta;
+  int ctas;
   int slots;
   int parts;      // most parts an item has
   // (all key tiles together stay below 2^31)
   __host__ __device__ __forceinline__ int first(int item) const {
-    return static_cast<uint32_t>(item * tiles) / static_cast<uint32_t>(per_cta);
+    return per_cta(item * tiles.d);
   }
   __host__ __device__ __forceinline__ int parts_of(int item) const {
-    return slots * (static_cast<int>(static_cast<uint32_t>((item + 1) * tiles - 1) / static_cast<uint32_t>(per_cta)) -
-                    first(item) + 1);
+    return slots * (static_cast<int>(per_cta((item + 1) * tiles.d - 1)) - first(item) + 1);
   }
 };
 // The sequences' own keys: items (sequence, key head, tile of rows), each cut
 // evenly into `splits`, a block each, which leaves `slots` parts.
 struct PaOwn {
-  int row_tiles, tile_rows, tile_keys, splits, slots, parts;
+  FastDiv row_tiles, splits;
+  int tile_rows, tile_keys, slots, parts;
 };
 
 struct PaArgs {
   const void* k;
   const void* v;
   long page_stride, row_stride, head_stride;
-  int n_pages, hkv;
-  FastDiv page_rows;
+  int n_pages;
+  FastDiv hkv, page_rows;
   const void* q;
   long ldq;
   void* out;
@@ -128,19 +129,19 @@ __device__ __forceinline__ int visible(const PaArgs& a, bool prefix, const PaRow
 struct PaRun {
   int item, tile, left;  // the next key tile and how many are left
   __device__ __forceinline__ PaRun(const PaPrefix& p, int hkv, int cta) {
-    const uint32_t at = static_cast<uint32_t>(cta) * static_cast<uint32_t>(p.per_cta);
-    const uint32_t all = static_cast<uint32_t>(hkv) * p.row_tiles * p.tiles;
-    left = at < all ? static_cast<int>(min(all - at, static_cast<uint32_t>(p.per_cta))) : 0;
-    item = p.tiles ? at / static_cast<uint32_t>(p.tiles) : 0;
-    tile = static_cast<int>(at - static_cast<uint32_t>(item) * p.tiles);
+    const uint32_t at = static_cast<uint32_t>(cta) * p.per_cta.d;
+    const uint32_t all = static_cast<uint32_t>(hkv) * p.row_tiles.d * p.tiles.d;
+    left = at < all ? static_cast<int>(min(all - at, p.per_cta.d)) : 0;
+    item = p.tiles(at);
+    tile = static_cast<int>(at - item * p.tiles.d);
   }
   __device__ __forceinline__ bool next(const PaArgs& a, int cta, PaPiece& w) {
     if (left <= 0) return false;
     const PaPrefix& p = a.prefix;
-    const int n = min(left, p.tiles - tile);
+    const int n = min(left, static_cast<int>(p.tiles.d) - tile);
     w.seq = -1;
-    w.head = static_cast<uint32_t>(item) / static_cast<uint32_t>(p.row_tiles);
-    w.row0 = (item - w.head * p.row_tiles) * p.tile_rows;
+    w.head = p.row_tiles(item);
+    w.row0 = (item - w.head * static_cast<int>(p.row_tiles.d)) * p.tile_rows;
     w.rows = a.b * a.seq_rows.d;
     w.part = (cta - p.first(item)) * p.slots;
     w.k0 = tile * p.tile_keys;
@@ -157,12 +158,11 @@ struct PaRun {
 __device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
   PaPiece w;
   const PaOwn& o = a.own;
-  const int tile = i % o.row_tiles;
-  i /= o.row_tiles;
-  w.head = i % a.hkv;
-  i /= a.hkv;
-  w.seq = i / o.splits;
-  const int split = i - w.seq * o.splits;
+  const int rest = o.row_tiles(i), tile = i - rest * static_cast<int>(o.row_tiles.d);
+  const int split_of = a.hkv(rest);
+  w.head = rest - split_of * static_cast<int>(a.hkv.d);
+  w.seq = o.splits(split_of);
+  const int splits = o.splits.d, split = split_of - w.seq * splits;
   w.row0 = tile * o.tile_rows;
   w.rows = a.seq_rows.d;
   w.part = a.prefix.parts + split * o.slots;
@@ -171,8 +171,8 @@ __device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
   const int last = a.group(min(w.row0 + o.tile_rows, w.rows) - 1);  // its query
   const int len = min(n, max(n - a.tq + last + 1, 0));
   const int tiles = (len + o.tile_keys - 1) / o.tile_keys;
-  w.k0 = static_cast<int>(static_cast<long>(tiles) * split / o.splits) * o.tile_keys;
-  w.k1 = min(static_cast<int>(static_cast<long>(tiles) * (split + 1) / o.splits) * o.tile_keys, len);
+  w.k0 = static_cast<int>(splits == 1 ? 0 : static_cast<long>(tiles) * split / splits) * o.tile_keys;
+  w.k1 = splits == 1 ? len : min(static_cast<int>(static_cast<long>(tiles) * (split + 1) / splits) * o.tile_keys, len);
   return w;
 }
 

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(P
   pdl_trigger();
   const int cta = blockIdx.x;
   if (cta < prefix_ctas) {
-    PaRun run(a.prefix, a.hkv, cta);
+    PaRun run(a.prefix, a.hkv.d, cta);
     PaPiece w;
     while (run.next(a, cta, w)) attend_piece<HD>(a, w, a.prefix.tile_rows, sh);
   } else {
@@ -398,7 +398,7 @@ struct WarpWork {
   PaRun run;
   int own;  // the own piece, or -1
   __device__ __forceinline__ WarpWork(const PaArgs& a, int prefix_ctas)
-      : run(a.prefix, a.hkv, blockIdx.x), own(static_cast<int>(blockIdx.x) - prefix_ctas) {
+      : run(a.prefix, a.hkv.d, blockIdx.x), own(static_cast<int>(blockIdx.x) - prefix_ctas) {
     if (own >= 0) run.left = 0;
   }
   __device__ __forceinline__ bool next(const PaArgs& a, PaPiece& w) {

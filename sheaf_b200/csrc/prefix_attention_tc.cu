@@ -20,8 +20,9 @@
 //   warp 11   looks through the tiles of V in which a row stops (below).
 // The softmax warps gather their rows of Q, those of the next piece while the
 // last products of this one run.
-// With at most 128 rows the two softmax groups take the same rows and the key
-// tiles in turn, each with an output of its own (two parts).
+// With at most 128 rows and several key tiles a block, the two softmax groups
+// take the same rows and the key tiles in turn, each with an output of its own
+// (two parts).
 // TMEM: S_0, S_1 (128 columns each), O_0, O_1 (HD each).
 #include <algorithm>
 
@@ -99,7 +100,7 @@ struct Pieces {
   PaRun run;
   int own;
   __device__ __forceinline__ Pieces(const PaArgs& a, int prefix_ctas)
-      : run(a.prefix, a.hkv, blockIdx.x), own(static_cast<int>(blockIdx.x) - prefix_ctas) {}
+      : run(a.prefix, a.hkv.d, blockIdx.x), own(static_cast<int>(blockIdx.x) - prefix_ctas) {}
   __device__ __forceinline__ bool next(const PaArgs& a, PaPiece& w) {
     if (own < 0) return run.next(a, blockIdx.x, w);
     if (own == 0x7fffffff) return false;
@@ -115,12 +116,16 @@ struct Pieces {
 // to the rows that see them at the end. (A row that sees no key of the piece
 // is dropped by its l = 0.) All lanes of a warp get the answer.
 __device__ __forceinline__ int care_of(const PaArgs& a, const PaPiece& w, int tile_rows) {
-  int care = w.k1;
   const int rows = min(tile_rows, w.rows - w.row0);
+  if (w.seq >= 0) {  // successive queries of one sequence: each sees one key more, or as many
+    const int seen = visible(a, false, row_of(a, w, w.row0));
+    return min(max(seen, w.k0 + 1), w.k1);
+  }
+  int care = w.k1;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {  // 256 rows; the loads are in flight together
     const int i = min(n * 32 + static_cast<int>(threadIdx.x % 32), rows - 1);
-    const int seen = visible(a, w.seq < 0, row_of(a, w, w.row0 + i));
+    const int seen = visible(a, true, row_of(a, w, w.row0 + i));
     if (seen > w.k0) care = min(care, seen);
   }
   return __reduce_min_sync(0xffffffffu, care);
@@ -188,7 +193,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   const uint32_t tmem = *tmem_slot;
   Pieces pieces(a, prefix_ctas);
   PaPiece w;
-  const int tile_rows = static_cast<int>(blockIdx.x) < prefix_ctas ? a.prefix.tile_rows : a.own.tile_rows;
+  const bool of_prefix = static_cast<int>(blockIdx.x) < prefix_ctas;
+  const int tile_rows = of_prefix ? a.prefix.tile_rows : a.own.tile_rows;
+  // one row tile, whose key tiles go to the two softmax groups in turn
+  const bool deal = (of_prefix ? a.prefix.slots : a.own.slots) == 2;
 
   if (warp >= kSoftWarps) regs_down<kOtherRegs>();
   if (warp == kSoftWarps + 1 || warp == kSoftWarps + 2) {
@@ -255,15 +263,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         for (int i = rows * CH + lane; i < kKeys * CH; i += 32)
           *reinterpret_cast<uint4*>(tile + chunk_at(i / CH, i % CH)) = make_uint4(0u, 0u, 0u, 0u);
         if (care < j0 + rows) {
-          const auto odd = [](uint32_t x) {  // one of two bf16 is no number
-            return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-          };
-          bool any = false;
-#pragma unroll 4
+          // an exponent of all ones carries into the bit above
+          const auto odd = [](uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; };
+          uint32_t carry = 0;
+#pragma unroll 8
           for (int i = lane; i < rows * CH; i += 32) {
             const uint4 u = *reinterpret_cast<const uint4*>(tile + chunk_at(i / CH, i % CH));
-            any |= odd(u.x) || odd(u.y) || odd(u.z) || odd(u.w);
+            carry |= odd(u.x) | odd(u.y) | odd(u.z) | odd(u.w);
           }
+          const bool any = (carry & 0x80008000u) != 0;
           if (__any_sync(0xffffffffu, any)) {
             int* bad = reinterpret_cast<int*>(sm + L::kBad);
             volatile int* found = reinterpret_cast<volatile int*>(sm + L::kFound);
@@ -359,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     while (ok && pieces.next(a, w)) {
       if (w.k1 <= w.k0) continue;
       const int n = (w.k1 - w.k0 + kKeys - 1) / kKeys;
-      if (tile_rows == kRows) {
-        // one row tile: key tile j for softmax group j % 2
+      if (deal) {
+        // key tile j for softmax group j % 2
         for (int j = 0; j < min(n, 2); ++j) {
           if (!wait(&k_full[kst], kph) || !wait(&q_full[j], begun[j]++ & 1)) break;
           scores(j);
@@ -380,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         continue;
       }
-      const int tiles = w.row0 + kRows < w.rows ? 2 : 1;
+      const int tiles = tile_rows > kRows && w.row0 + kRows < w.rows ? 2 : 1;
       if (!wait(&k_full[kst], kph)) break;
       for (int x = 0; x < tiles; ++x) {
         if (!wait(&q_full[x], begun[x]++ & 1)) break;
@@ -410,7 +418,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // ---- softmax ---------------------------------------------------------
     regs_up<kSoftRegs>();
     const int x = warp / 4, quarter = warp % 4;
-    const bool deal = tile_rows == kRows;  // key tiles go to the two groups in turn
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + lanes + x * 128, tO = tmem + lanes + L::kTmemO + x * HD;
     const float sl = a.scale * 1.4426950408889634f;
@@ -434,22 +441,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const auto row_in = [&](const PaPiece& p) {
       Mine m;
       const int i = p.row0 + (deal ? 0 : x * kRows) + quarter * 32 + lane;
-      m.in = i < p.rows;
+      m.in = i < p.rows && (deal || x == 0 || tile_rows > kRows);
       m.tiles = (max(p.k1 - p.k0, 0) + kKeys - 1) / kKeys;
       if (deal)
         m.tiles = (m.tiles + 1 - x) / 2;
-      else if (x == 1 && p.row0 + kRows >= p.rows)
+      else if (x == 1 && (tile_rows == kRows || p.row0 + kRows >= p.rows))
         m.tiles = 0;
       m.none = false;
       m.seen = p.k1;  // a row that sees nothing is let go along, and dropped at the end
       m.at = 0;
       m.out_at = 0;
       long q_at = -1;
+      PaRow r;
       if (m.in) {
-        const PaRow r = row_of(a, p, i);
-        const int seen = visible(a, p.seq < 0, r);
-        m.none = seen <= p.k0;
-        if (!m.none) m.seen = min(seen, p.k1);
+        r = row_of(a, p, i);
         m.at = r.token * a.hq + r.h;
         m.out_at = r.token * a.ldo + static_cast<long>(r.h) * HD;
         q_at = r.token * a.ldq + static_cast<long>(r.h) * HD;
@@ -467,6 +472,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
       }
       cp_async_commit();
+      if (m.in) {
+        const int seen = visible(a, p.seq < 0, r);
+        m.none = seen <= p.k0;
+        if (!m.none) m.seen = min(seen, p.k1);
+      }
       return m;
     };
     const auto announce_q = [&](const Mine& m) {
@@ -611,11 +621,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           their_at[k] = __shfl_sync(0xffffffffu, row_at, 8 * k + lane / 4);
           their_scale[k] = __shfl_sync(0xffffffffu, scale, 8 * k + lane / 4);
         }
+        uint32_t ahead[16];
+        tmem_ld16(tO, ahead);
 #pragma unroll 1
         for (int cc = 0; cc < HD / 16; ++cc) {
           uint32_t v[16];
-          tmem_ld16(tO + cc * 16, v);
           tmem_wait_ld();
+#pragma unroll
+          for (int t = 0; t < 16; ++t) v[t] = ahead[t];
+          if (cc + 1 < HD / 16) tmem_ld16(tO + (cc + 1) * 16, ahead);
           if (some && l != 0.f) {
 #pragma unroll
             for (int t = 0; t < 16; ++t)
