@@ -182,20 +182,208 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& 
   }
 }
 
-// Blocks [0, prefix blocks) take runs of the prefix, the others own pieces.
+// The same for 64 rows, 16 a warp: a lane computes the scores of 4 rows with 4
+// keys, then 4 rows of HD / 8 output columns, so that each 16 bytes read from
+// shared memory serve 8 or more multiply-adds and these bound the kernel.
+// (With 4 rows a warp the shared-memory reads do: 8 x 41 queries of 4 heads of
+// 128 behind 10565 keys took 590 us, this TODO.)
+constexpr int kWideRows = 64;
+
+template <int HD>
+struct WideShared {
+  float q[kWideRows][HD + 4];
+  float k[2][kKeys][HD + 4];
+  float v[2][kKeys][HD];
+  float p[kThreads / 32][kKeys][16];
+};
+
+template <int HD>
+__device__ void attend_wide(const PaArgs& a, const PaPiece& w, WideShared<HD>& sh) {
+  constexpr int Q = HD / 32;  // groups of 4 output columns a lane has
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int rg = lane / 8, kg = lane % 8;  // rows 4 rg .., keys kg + 8 i
+  const int* table = table_of(a, w);
+
+  PaRow row[4];
+  int seen[4], most = 0, least = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = w.row0 + warp * 16 + rg * 4 + r;
+    seen[r] = w.k1;  // a row of no one sees all and is not stored
+    if (i < w.rows) {
+      row[r] = row_of(a, w, i);
+      seen[r] = min(visible(a, w.seq < 0, row[r]), w.k1);
+      most = max(most, seen[r]);
+      if (seen[r] > w.k0) least = min(least, seen[r]);
+    }
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int k1 = __syncthreads_or(most > w.k0) ? w.k1 : w.k0;  // shared memory is free, too
+
+  constexpr int CH = HD / 4;  // vectors of a row
+  for (int i = tid; i < kWideRows * CH; i += kThreads) {
+    const int r = w.row0 + i / CH, c = i % CH * 4;
+    const bool in = r < w.rows;
+    long at = 0;
+    if (in) {
+      const PaRow x = row_of(a, w, r);
+      at = x.token * a.ldq + static_cast<long>(x.h) * HD + c;
+    }
+    cp_async16(smem_u32(&sh.q[i / CH][c]), static_cast<const float*>(a.q) + at, in);
+  }
+  const auto load = [&](int stage, int j0) {
+#pragma unroll 4
+    for (int i = tid; i < kKeys * CH; i += kThreads) {
+      const int j = i / CH, c = i % CH * 4;
+      const bool in = j0 + j < k1;
+      const long at = in ? key_offset(a, table, j0 + j) + w.head * a.head_stride + c : 0;
+      cp_async16(smem_u32(&sh.k[stage][j][c]), static_cast<const float*>(a.k) + at, in);
+      cp_async16(smem_u32(&sh.v[stage][j][c]), static_cast<const float*>(a.v) + at, in);
+    }
+    cp_async_commit();
+  };
+
+  float m[4], l[4], o[4][Q][4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < Q; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][c][e] = 0.f;
+  }
+  load(0, w.k0);
+  int stage = 0;
+  for (int j0 = w.k0; j0 < k1; j0 += kKeys, stage ^= 1) {
+    if (j0 + kKeys < k1) {
+      load(stage ^ 1, j0 + kKeys);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    if (j0 < most) {
+      float s[4][4] = {};  // row, key
+#pragma unroll 4
+      for (int c = 0; c < HD; c += 4) {
+        float4 q[4], k[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r] = *reinterpret_cast<const float4*>(&sh.q[warp * 16 + rg * 4 + r][c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(&sh.k[stage][kg + 8 * i][c]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[r][i] = fmaf(q[r].x, k[i].x, fmaf(q[r].y, k[i].y, fmaf(q[r].z, k[i].z, fmaf(q[r].w, k[i].w, s[r][i]))));
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[r][i] = j0 + kg + 8 * i < seen[r] ? s[r][i] * a.scale : -INFINITY;
+          t = fmaxf(t, s[r][i]);
+        }
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+        const float mn = fmaxf(m[r], t);
+        const float f = mn == -INFINITY ? 1.f : expf(m[r] - mn);
+        l[r] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[r][i] = mn == -INFINITY ? 0.f : expf(s[r][i] - mn);
+          l[r] += s[r][i];
+        }
+        m[r] = mn;
+#pragma unroll
+        for (int c = 0; c < Q; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[r][c][e] *= f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(&sh.p[warp][kg + 8 * i][rg * 4]) = make_float4(s[0][i], s[1][i], s[2][i], s[3][i]);
+      __syncwarp();
+      // where some row stops inside the tile, a key that it does not see must
+      // not reach it, whatever its values hold (0 * NaN)
+      const bool care = j0 + kKeys > least;
+      const int n = min(kKeys, k1 - j0);
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const float4 p4 = *reinterpret_cast<const float4*>(&sh.p[warp][j][rg * 4]);
+        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+        for (int c = 0; c < Q; ++c) {
+          const float4 v4 = *reinterpret_cast<const float4*>(&sh.v[stage][j][c * 32 + kg * 4]);
+          const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (care && j0 + j >= seen[r]) continue;
+              o[r][c][e] = fmaf(p[r], v[e], o[r][c][e]);
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float sum = l[r];
+#pragma unroll
+    for (int x = 4; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (w.row0 + warp * 16 + rg * 4 + r >= w.rows) continue;
+    const long at = row[r].token * a.hq + row[r].h;
+    if (a.direct) {
+      const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      float* out = static_cast<float*>(a.out) + row[r].token * a.ldo + static_cast<long>(row[r].h) * HD + kg * 4;
+#pragma unroll
+      for (int c = 0; c < Q; ++c)
+        *reinterpret_cast<float4*>(out + c * 32) =
+            make_float4(o[r][c][0] * f, o[r][c][1] * f, o[r][c][2] * f, o[r][c][3] * f);
+      if (a.lse && kg == 0) a.lse[at] = m[r] + logf(sum);
+    } else {
+      const long slot = static_cast<long>(w.part) * a.b * a.tq * a.hq + at;
+      if (kg == 0) a.part_ml[slot] = make_float2(m[r], sum);
+      if (sum != 0.f)
+#pragma unroll
+        for (int c = 0; c < Q; ++c)
+          *reinterpret_cast<float4*>(a.part_o + slot * HD + c * 32 + kg * 4) =
+              make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+    }
+  }
+}
+
+// Blocks [0, prefix blocks) take runs of the prefix, the others own pieces,
+// with 16 or 64 rows a block as the segment's tiles have.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PaArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SimtShared<HD>& sh = *reinterpret_cast<SimtShared<HD>*>(smem_raw);
+  WideShared<HD>& wide = *reinterpret_cast<WideShared<HD>*>(smem_raw);
   pdl_wait();
   pdl_trigger();
   const int cta = blockIdx.x;
+  PaPiece w;
   if (cta < a.prefix.ctas) {
     PaRun run(a.prefix, a.hkv.d, cta);
-    PaPiece w;
-    while (run.next(a, cta, w)) attend_piece<HD>(a, w, sh);
+    while (run.next(a, cta, w)) {
+      if (a.prefix.tile_rows == kWideRows)
+        attend_wide<HD>(a, w, wide);
+      else
+        attend_piece<HD>(a, w, sh);
+    }
   } else {
-    attend_piece<HD>(a, own_piece(a, cta - a.prefix.ctas), sh);
+    w = own_piece(a, cta - a.prefix.ctas);
+    if (a.own.tile_rows == kWideRows)
+      attend_wide<HD>(a, w, wide);
+    else
+      attend_piece<HD>(a, w, sh);
   }
 }
 
@@ -324,7 +512,8 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   };
   const auto rows_of = [](Kernel k, long rows) {
     if (k == kTc) return rows > 128 ? 256 : 128;
-    return k == kSimt || rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+    if (k == kSimt) return rows <= 16 ? kRows : kWideRows;
+    return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
   };
   const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : (k == kWarp ? 16 : kKeys)); };
   const long own_capacity = static_cast<long>(d.max_pages) * d.cache.page_rows;
@@ -387,11 +576,12 @@ namespace {
 
 template <int HD>
 int simt(const PaArgs& a, int own_ctas, cudaStream_t s) {
-  constexpr size_t smem = sizeof(SimtShared<HD>);
+  const bool wide = (a.prefix.ctas > 0 && a.prefix.tile_rows == kWideRows) || (own_ctas > 0 && a.own.tile_rows == kWideRows);
+  const size_t smem = wide ? sizeof(WideShared<HD>) : sizeof(SimtShared<HD>);
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(attn_simt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
+                             static_cast<int>(std::max(sizeof(WideShared<HD>), sizeof(SimtShared<HD>)))) != cudaSuccess)
       return SB_OPERR_LAUNCH;
     attr = true;
   }
