@@ -234,7 +234,9 @@ SB_API int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld
  * q, out [b * tq, h_q * head_dim] (row strides ldq, ldo; query head h reads
  * key head h / (h_q / n_heads)) in the cache's element type; lse f32
  * [b * tq, h_q], or NULL. A query that sees no key (lens[s] < 0 marks an idle
- * slot) gets a zero row and lse = -inf. prefix_len = 0 is plain attention
+ * slot) gets a zero row and lse = -inf; so does one all of whose scores are
+ * -inf. An infinite value makes its column inf or NaN for the queries that see
+ * its key, and for no others. prefix_len = 0 is plain attention
  * over a paged cache, max_pages = 0 attention to the prefix alone. lens[s]
  * beyond its table counts as the table's capacity and a page outside the
  * cache as page 0; sb_op_device_error then reports 2. scale > 0. q, out and

@@ -18,6 +18,12 @@
 // best logit from below, so only what the few threads saw whose own best
 // reaches that bound is looked at again (from L2, by all threads), and only
 // logits that reach it become candidates: about 64 ln(64 / (64 - k)) of them.
+//
+// Reading the logits bounds it: 8192 x 50304 bf16, 824 MB, take 126 us at the
+// measured copy rate, and 152 us without alternatives, 184 with 8 (0.68). What
+// is left: the exponentials alone take 0.57 of the time on their unit, and a
+// block does not read while it joins a row's statistics and looks up the
+// alternatives. The VJP reads and writes once: 4096 x 50304 in 147 us, 0.86.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -186,7 +186,8 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& 
 // keys, then 4 rows of HD / 8 output columns, so that each 16 bytes read from
 // shared memory serve 8 or more multiply-adds and these bound the kernel.
 // (With 4 rows a warp the shared-memory reads do: 8 x 41 queries of 4 heads of
-// 128 behind 10565 keys took 590 us, this TODO.)
+// 128 behind 10565 keys took 590 us; this takes 308, 23 TFLOP/s, with 8 warps
+// an SM, too few to cover the latency of the arithmetic.)
 constexpr int kWideRows = 64;
 
 template <int HD>
@@ -501,9 +502,10 @@ long ceil_div(long a, long b) { return (a + b - 1) / b; }
 bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const long G = d.h_q / d.cache.n_heads, hkv = d.cache.n_heads;
   const long prefix_rows = static_cast<long>(d.b) * d.tq * G, own_rows = d.tq * G;
-  // tcgen05 tiles for more than 64 rows; from 17 rows on where every SM gets
-  // some 128-key tiles to spread a block's start and end over (8 x 4 rows
-  // behind 131072 keys: TODO us, the warp-level kernel 147; behind TODO).
+  // Up to 16 rows a warp each; tcgen05 tiles for more than 64, and from 17 on
+  // where a hundred key tiles spread the start and end of its blocks: 32 rows of
+  // 8 key heads behind 131072 keys 117 us, the warp-level kernel 147; behind
+  // 8192, 27 and 32; 64 rows behind 8192, 28 and 41; behind 1024 the same.
   const auto choose = [&](long rows, long items, long keys) {
     if (d.cache.elem == SB_ELEM_F32) return kSimt;
     if (rows <= 16) return kWarp;

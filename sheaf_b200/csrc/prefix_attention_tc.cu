@@ -3,6 +3,13 @@
 // multiply-adds a byte, so from about 64 rows the products and exponentials
 // bound it, not the reading.
 //
+// What bounds it: per key tile and SM, 32 UMMAs of 64 cycles against 32768
+// exponentials at 16 a cycle, 2050 cycles each; measured 3690, because a row
+// tile's softmax (1620) and its products with their commits and waits (2070)
+// follow one another, with the other row tile half a period behind. 512 x 32
+// queries behind 16384 keys, 137 GFLOP: 142 us, 0.60 of the measured bf16 peak.
+// (7 of 16 exponentials as polynomials in FMAs: 4140 cycles.)
+//
 // A block takes up to 256 rows, two tiles of 128, against tiles of 128 keys;
 // 12 warps:
 //   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row; P goes back to TMEM as bf16 over the
@@ -14,9 +21,10 @@
 //             While one row tile's softmax runs, the other's products do.
 //   warps 9, 10  copy K, V through the page tables: a tiled bulk copy for each
 //             run of rows that lies in one page whatever the tile's place (the
-//             largest power of two that divides the page), a lane each. One
-//             warp for both had K wait for room for V and took 5200 cycles a
-//             tile where two take TODO.
+//             largest power of two that divides the page), a lane each. (With
+//             one warp for both, K waited behind V for room: 512 queries of 32
+//             heads behind 16384 keys took 271 us, with two 210. 16-byte
+//             asynchronous copies by 96 threads before that: 446.)
 //   warp 11   looks through the tiles of V in which a row stops (below).
 // The softmax warps gather their rows of Q, those of the next piece while the
 // last products of this one run.
@@ -498,98 +506,102 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int seen = mine.seen;
       const int least = __reduce_min_sync(0xffffffffu, seen);
       float ref = -INFINITY, l = 0.f;
+      bool open = true;  // some row has no reference yet: every score it has seen is -inf
       for (int j = 0; j < mine.tiles; ++j, ++c) {
-          const int j0 = w.k0 + (deal ? 2 * j + x : j) * kKeys;
-          if (!wait(&s_full[x], c & 1)) break;
-          const bool part = j0 + kKeys > least;  // some row stops in this tile
-          // Scores go to p = 2^(s - ref) without their maximum being looked
-          // for. Only at a piece's first tile (next loop) and where a row's sum
-          // passes 2^15 is the reference raised; in the latter case O is
-          // rescaled and p taken again from the scores, still in registers.
-          if (j == 0 || part) {
-            // keys that a row does not see get their scores out of the way
-            float mx = -INFINITY;
+        const int j0 = w.k0 + (deal ? 2 * j + x : j) * kKeys;
+        if (!wait(&s_full[x], c & 1)) break;
+        const bool part = j0 + kKeys > least;  // some row stops in this tile
+        // Scores go to p = 2^(s - ref) without their maximum being looked
+        // for. Only until every row has a reference (next loop; mostly at a
+        // piece's first tile) and where a row's sum passes 2^15 is it raised;
+        // in the latter case O is rescaled and p taken again from the scores,
+        // still in registers.
+        if (open || part) {
+          // keys that a row does not see get their scores out of the way
+          float mx = -INFINITY;
 #pragma unroll 1
-            for (int cc = 0; cc < 8; ++cc) {
-              uint32_t u[16];
-              tmem_ld16(tS + cc * 16, u);
-              tmem_wait_ld();
-              const int limit = seen - j0 - cc * 16;
-#pragma unroll
-              for (int t = 0; t < 16; ++t) {
-                if (t >= limit) u[t] = __float_as_uint(-INFINITY);
-                mx = fmaxf(mx, __uint_as_float(u[t]));
-              }
-              if (part) tmem_st16(tS + cc * 16, u);
-            }
-            if (part) tmem_wait_st();
-            if (j == 0) ref = mx * sl;
-          }
-          uint32_t v[4][32];
-          const float2 sl2 = make_float2(sl, sl);
-          float2 sum[2];
-          const auto exps = [&](int cc) {
-            const float sub = ref == -INFINITY ? 0.f : ref;
-            const float2 sub2 = make_float2(-sub, -sub);
-            uint32_t pk[16];
+          for (int cc = 0; cc < 8; ++cc) {
+            uint32_t u[16];
+            tmem_ld16(tS + cc * 16, u);
+            tmem_wait_ld();
+            const int limit = seen - j0 - cc * 16;
 #pragma unroll
             for (int t = 0; t < 16; ++t) {
-              const float2 y = __ffma2_rn(
-                  make_float2(__uint_as_float(v[cc][2 * t]), __uint_as_float(v[cc][2 * t + 1])), sl2, sub2);
-              const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-              sum[t & 1] = __fadd2_rn(sum[t & 1], p);
-              pk[t] = pack_bf16x2(p.x, p.y);
+              if (t >= limit) u[t] = __float_as_uint(-INFINITY);
+              mx = fmaxf(mx, __uint_as_float(u[t]));
             }
-            tmem_st16(tS + cc * 16, pk);  // over scores that have been read
-          };
-          const auto total = [&] { return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y); };
-          // 32 scores at a time, the next on their way meanwhile
-          sum[0] = sum[1] = make_float2(0.f, 0.f);
-          tmem_ld32(tS, v[0]);
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            tmem_wait_ld();
-            if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, v[cc + 1]);
-            exps(cc);
+            if (part) tmem_st16(tS + cc * 16, u);
           }
-          float tile_l = total();
-          // A NaN is left as it is. A row without a reference sees no key so
-          // far, and so none later either.
-          if (__builtin_expect(__any_sync(0xffffffffu, tile_l > 32768.f), 0)) {
-            float m[2] = {ref, -INFINITY};
+          if (part) tmem_wait_st();
+          if (open) {
+            if (ref == -INFINITY) ref = mx * sl;
+            open = __any_sync(0xffffffffu, ref == -INFINITY && j0 + kKeys < seen);
+          }
+        }
+        uint32_t v[4][32];
+        const float2 sl2 = make_float2(sl, sl);
+        float2 sum[2];
+        const auto exps = [&](int cc) {
+          const float sub = ref == -INFINITY ? 0.f : ref;
+          const float2 sub2 = make_float2(-sub, -sub);
+          uint32_t pk[16];
 #pragma unroll
-            for (int cc = 0; cc < 4; ++cc)
+          for (int t = 0; t < 16; ++t) {
+            const float2 y = __ffma2_rn(
+                make_float2(__uint_as_float(v[cc][2 * t]), __uint_as_float(v[cc][2 * t + 1])), sl2, sub2);
+            const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            sum[t & 1] = __fadd2_rn(sum[t & 1], p);
+            pk[t] = pack_bf16x2(p.x, p.y);
+          }
+          tmem_st16(tS + cc * 16, pk);  // over scores that have been read
+        };
+        const auto total = [&] { return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y); };
+        // 32 scores at a time, the next on their way meanwhile
+        sum[0] = sum[1] = make_float2(0.f, 0.f);
+        tmem_ld32(tS, v[0]);
 #pragma unroll
-              for (int t = 0; t < 32; t += 2) {
-                m[0] = fmaxf(m[0], __uint_as_float(v[cc][t]) * sl);
-                m[1] = fmaxf(m[1], __uint_as_float(v[cc][t + 1]) * sl);
-              }
-            const float mx = fmaxf(m[0], m[1]);
-            const float f = mx == -INFINITY ? 1.f : ex2_approx(ref - mx);
-            ref = mx;
-            l *= f;
-            if (j > 0) {
-              if (!wait(&o_full[x], (c - 1) & 1)) break;
+        for (int cc = 0; cc < 4; ++cc) {
+          tmem_wait_ld();
+          if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, v[cc + 1]);
+          exps(cc);
+        }
+        float tile_l = total();
+        // A NaN is left as it is.
+        if (__builtin_expect(__any_sync(0xffffffffu, tile_l > 32768.f), 0)) {
+          float m[2] = {ref, -INFINITY};
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+            for (int t = 0; t < 32; t += 2) {
+              m[0] = fmaxf(m[0], __uint_as_float(v[cc][t]) * sl);
+              m[1] = fmaxf(m[1], __uint_as_float(v[cc][t + 1]) * sl);
+            }
+          const float mx = fmaxf(m[0], m[1]);
+          const float f = mx == -INFINITY ? 1.f : ex2_approx(ref - mx);
+          ref = mx;
+          l *= f;
+          if (j > 0) {
+            if (!wait(&o_full[x], (c - 1) & 1)) break;
 #pragma unroll 1
-              for (int cc = 0; cc < HD / 16; ++cc) {
-                uint32_t u[16];
-                tmem_ld16(tO + cc * 16, u);
-                tmem_wait_ld();
+            for (int cc = 0; cc < HD / 16; ++cc) {
+              uint32_t u[16];
+              tmem_ld16(tO + cc * 16, u);
+              tmem_wait_ld();
 #pragma unroll
-                for (int t = 0; t < 16; ++t) u[t] = __float_as_uint(__uint_as_float(u[t]) * f);
-                tmem_st16(tO + cc * 16, u);
-              }
+              for (int t = 0; t < 16; ++t) u[t] = __float_as_uint(__uint_as_float(u[t]) * f);
+              tmem_st16(tO + cc * 16, u);
             }
-            sum[0] = sum[1] = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) exps(cc);
-            tile_l = total();
           }
-          l += tile_l;
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[x]);
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) exps(cc);
+          tile_l = total();
+        }
+        l += tile_l;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
       }
       if (!ok) break;
       if (mine.none) {

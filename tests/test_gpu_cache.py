@@ -382,6 +382,25 @@ def test_attention_keeps_unseen_keys_out(kind, cuda):
     assert np.isnan(got[1][:, 5]).all() and np.array_equal(np.delete(got[1], 5, 1), np.delete(clean[1], 5, 1))
 
 
+@pytest.mark.parametrize("kind,seqs,prefix", [("bf16", 3, 20000), ("bf16", 20, 1500), ("bf16", 70, 20000),
+                                              ("f32", 3, 20000), ("f32", 70, 20000)])
+def test_attention_keys_at_minus_infinity(kind, seqs, prefix, cuda):
+    """Seen keys with a score of -inf weigh nothing, however many come first and however low the others' scores."""
+    a = _Attend(kind, 8, 8, 32, 16, prefix, [5] * seqs, 1, cuda)
+    q = a.q.view(-1, 8, 32)
+    q[..., 0], q[..., 1] = 1.0, 32.0
+    a.k[..., 1] = -100.0
+    closed = np.arange(len(a.prefix_table)) % 32 < 20   # 320 keys of every 512
+    closed[-1] = False
+    a.k[_i(a.prefix_table[closed], cuda).long(), ..., 0] = float("-inf")
+    got, lse = a()
+    for r in (0, seqs // 2, seqs - 1):
+        open_ = a.prefix_table[~closed]
+        one = _attend64(_f64(a.q)[r:r + 1], _f64(a.k), _f64(a.v), open_, a.prefix - 16 * int(closed.sum()),
+                        a.table[r:r + 1], [5], 1, a.scale, 16)
+        _check_attention(kind, got[r:r + 1], lse[r:r + 1], one, 32)
+
+
 def test_attention_reports_indices_outside(cuda):
     a = _Attend("bf16", 4, 2, 64, 16, 40, [20, 16], 1, cuda)
     a.lens = np.array([20, 33])  # two pages hold 32
