@@ -527,8 +527,9 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   p.own.tile_keys = keys_of(p.own_kernel);
   const long prefix_row_tiles = ceil_div(prefix_rows, p.prefix.tile_rows);
   const long own_row_tiles = ceil_div(own_rows, p.own.tile_rows);
-  const long prefix_tiles = ceil_div(d.prefix_len, p.prefix.tile_keys), own_tiles = ceil_div(own_capacity, p.own.tile_keys);
-  const long prefix_work = hkv * prefix_row_tiles * prefix_tiles;
+  const long own_tiles = ceil_div(own_capacity, p.own.tile_keys);
+  long prefix_tiles = ceil_div(d.prefix_len, p.prefix.tile_keys);
+  long prefix_work = hkv * prefix_row_tiles * prefix_tiles;
   const long own_items = d.b * hkv * own_row_tiles, own_work = own_items * own_tiles;
   // Key tiles that a block takes: at least 2, and enough that all blocks of a
   // launch are resident at once.
@@ -537,8 +538,41 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
     const long blocks = k == kTc ? 1 : (k == kWarp ? warp_blocks_per_sm(d.cache.head_dim) : 2);
     return std::max(k == kWarp ? 4L : 2L, ceil_div(work, blocks * num_sms_cached()));
   };
-  const long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
   const long own_quota = quota(p.own_kernel, own_work + (together ? prefix_work : 0));
+  long prefix_quota = quota(p.prefix_kernel, prefix_work + (together ? own_work : 0));
+  if (p.prefix_kernel == kTc && prefix_work > 0 && !together) {
+    long sms = num_sms_cached();
+    // Own keys of one-warp blocks run beside the prefix: a tcgen05 block costs
+    // about 10 us beyond its key tiles, so it takes more of them on fewer SMs,
+    // and the own keys' blocks fill the others and, as they come free, these.
+    // A 256-row tile costs an SM as much as 7 of the warps' 16-key tiles; about
+    // a third of the own capacity is counted, since lengths are on the device
+    // and too many SMs cost less than too few. (64 x 32 queries behind 8192
+    // shared and up to 512 own keys 49 -> 41 us, counting a sixth 48; 100 of
+    // them behind 20000, 96 -> 73.) Beyond 24 tiles, or an eighth more than all
+    // SMs would give, nothing is gained (512 behind 16384 and up to 256: 201 at
+    // half as many again, 198 here), and the prefix could end last (512 behind
+    // 400 and up to 600: 136 us, 282 without this limit).
+    if (p.own_kernel == kWarp && own_work > 0) {
+      const long own = own_work * 256 / p.prefix.tile_rows / 20;
+      sms = std::max(1L, sms * prefix_work / (prefix_work + own));
+      prefix_quota = std::min(std::max(2L, ceil_div(prefix_work, sms)), std::max(24L, prefix_quota * 9 / 8));
+      sms = std::max(sms, ceil_div(prefix_work, prefix_quota));
+    }
+    // Runs that end with an item, where they are not much longer: a second
+    // piece costs a block 2.5 tiles (64 queries as above, 8 tiles a block 45
+    // us, 7 and 9: 49 and 50; 512 and next to no own keys, 64 tiles 135, 56:
+    // 140, under the power cap 151 and 158).
+    const long each = sms / (hkv * prefix_row_tiles);  // blocks an item
+    if (each > 0) {
+      const long even = std::max(2L, ceil_div(prefix_tiles, each));
+      if (8 * even <= 9 * prefix_quota + 20) {
+        prefix_quota = even;
+        prefix_tiles = ceil_div(prefix_tiles, even) * even;
+        prefix_work = hkv * prefix_row_tiles * prefix_tiles;
+      }
+    }
+  }
   if (prefix_work + prefix_quota > 0x7fffffffL) return false;  // counted in 32 bits
   p.prefix.row_tiles = FastDiv::of(static_cast<uint32_t>(prefix_row_tiles));
   p.prefix.tiles = FastDiv::of(static_cast<uint32_t>(std::max(1L, prefix_tiles)));
@@ -552,6 +586,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   p.own.slots = p.own_kernel == kTc && p.own.tile_rows == 128 && own_tiles >= 2 * splits ? 2 : 1;
   p.prefix.parts = prefix_work ? static_cast<int>((prefix_tiles - 1) / prefix_quota + 2) : 0;
   if (prefix_work && prefix_quota % prefix_tiles == 0) p.prefix.parts = 1;  // whole items a block
+  if (prefix_work && prefix_tiles % prefix_quota == 0) p.prefix.parts = static_cast<int>(prefix_tiles / prefix_quota);
   p.prefix.parts *= p.prefix.slots;
   p.own.row_tiles = FastDiv::of(static_cast<uint32_t>(own_row_tiles));
   p.own.splits = FastDiv::of(static_cast<uint32_t>(std::max(1L, splits)));
@@ -612,8 +647,12 @@ size_t align16(size_t n) { return (n + 15) & ~size_t{15}; }
 
 }  // namespace
 
-int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
-int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s);
+// `early`: a kernel that starts beside the one before it on the stream, which
+// writes nothing that it reads or writes and whose blocks all have started, so
+// its own predecessors have completed. One block waits for that kernel at its
+// end: whoever waits for the second then has the first's results as well.
+int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
+int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
 int attn_tc(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s);
 
 size_t prefix_attention_workspace_bytes(const PrefixAttnDesc& d) {
@@ -664,24 +703,15 @@ int prefix_attention(const PrefixAttnDesc& d, void* ws, size_t, cudaStream_t s, 
   const bool f32 = d.cache.elem == SB_ELEM_F32;
   int rc = 0;
   if (!f32) {
-    // A kernel takes both segments or one; parts of the two are apart, so a
-    // tcgen05 launch starts beside the one before it.
-    const auto of = [&](Kernel k, int& prefix, int& own) {
-      prefix = p.prefix_kernel == k ? a.prefix.ctas : 0;
-      own = p.own_kernel == k ? p.own_ctas : 0;
-      return prefix + own > 0;
+    // One launch for both segments, or the own keys' beside the prefix's: their
+    // parts are apart, so the second starts once all blocks of the first have.
+    const auto attend = [&](Kernel k, int prefix, int own, bool early) {
+      if (prefix + own == 0) return 0;
+      return (k == kTc ? attn_tc : (k == kMma ? attn_mma : attn_warp))(a, hd, prefix, own, early, s);
     };
-    int prefix, own;
-    bool before = false;
-    if (of(kWarp, prefix, own)) {
-      rc = attn_warp(a, hd, prefix, own, s);
-      before = true;
-    }
-    if (!rc && of(kMma, prefix, own)) {
-      rc = attn_mma(a, hd, prefix, own, s);
-      before = true;
-    }
-    if (!rc && of(kTc, prefix, own)) rc = attn_tc(a, hd, prefix, own, before, s);
+    const bool together = p.prefix_kernel == p.own_kernel;
+    rc = attend(p.prefix_kernel, a.prefix.ctas, together ? p.own_ctas : 0, false);
+    if (!rc && !together) rc = attend(p.own_kernel, 0, p.own_ctas, a.prefix.ctas > 0);
   } else
     rc = hd == 32 ? simt<32>(a, p.own_ctas, s) : (hd == 64 ? simt<64>(a, p.own_ctas, s) : simt<128>(a, p.own_ctas, s));
   if (rc || a.direct) return rc;

@@ -145,7 +145,8 @@ struct PaRun {
     w.rows = a.b * a.seq_rows.d;
     w.part = (cta - p.first(item)) * p.slots;
     w.k0 = tile * p.tile_keys;
-    w.k1 = min((tile + n) * p.tile_keys, a.prefix_len);
+    // (an item's tiles may be counted beyond its end, to a multiple of a run)
+    w.k1 = static_cast<int>(min(static_cast<long>(tile + n) * p.tile_keys, static_cast<long>(a.prefix_len)));
     left -= n;
     tile = 0;
     ++item;
@@ -198,6 +199,17 @@ bool cache_map(void* map, const void* base, const PaArgs& a, int hd);
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+// ... of data that is read once
+__device__ __forceinline__ uint64_t read_once_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
+               "r"(read ? 16 : 0), "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

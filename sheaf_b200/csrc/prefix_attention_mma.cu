@@ -369,11 +369,12 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, int tile_rows, M
 }
 
 // Blocks [0, prefix blocks) take runs of the prefix, the others own pieces.
+// `early`: see attn_mma's declaration.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(PaArgs a, int prefix_ctas) {
+__global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(PaArgs a, int prefix_ctas, int early) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   MmaShared<HD>& sh = *reinterpret_cast<MmaShared<HD>*>(smem_raw);
-  pdl_wait();
+  if (!early) pdl_wait();
   pdl_trigger();
   const int cta = blockIdx.x;
   if (cta < prefix_ctas) {
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(P
   } else {
     attend_piece<HD>(a, own_piece(a, cta - prefix_ctas), a.own.tile_rows, sh);
   }
+  if (early && cta == 0) pdl_wait();
 }
 
 // ---- one warp a piece: at most 16 rows -------------------------------------
@@ -414,14 +416,14 @@ struct WarpWork {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas) {
+__global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas, int early) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   WarpShared<HD>& sh = *reinterpret_cast<WarpShared<HD>*>(smem_raw);
   using bf = __nv_bfloat16;
   constexpr int CH = HD / 8, ST = kWarpStages;
   const int lane = threadIdx.x;
   const float sl = a.scale * 1.4426950408889634f;
-  pdl_wait();
+  if (!early) pdl_wait();
   pdl_trigger();
 
   // the copies' place in the work, ahead of the products'
@@ -431,6 +433,9 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
   int lj = 0;
   long off = 0;  // of key lj + lane % 16
   bool more = true;
+  // One block reads a key, and the prefix's, which many read, stay in L2 (64
+  // sequences beside a tcgen05 prefix of 8192 keys 44 -> 41 us).
+  const uint64_t once = read_once_policy();
   const auto locate = [&] {
     const int j = lj + (lane & 15);
     off = j < lw.k1 ? key_offset(a, table_of(a, lw), j) + static_cast<long>(lw.head) * a.head_stride : 0;
@@ -450,8 +455,8 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
         const long o = __shfl_sync(0xffffffffu, off, r) + c * 8;
         const bool in = lj + r < lw.k1;
         const uint32_t d = chunk_at<HD>(r, c);
-        cp_async16(sk + d, static_cast<const bf*>(a.k) + (in ? o : 0), in);
-        cp_async16(sv + d, static_cast<const bf*>(a.v) + (in ? o : 0), in);
+        cp_async16(sk + d, static_cast<const bf*>(a.k) + (in ? o : 0), in, once);
+        cp_async16(sv + d, static_cast<const bf*>(a.v) + (in ? o : 0), in, once);
       }
       lj += 16;
       if (lj < lw.k1) locate();
@@ -519,10 +524,11 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
     __syncwarp();  // bad is read before the next piece resets it
   }
   cp_async_wait<0>();
+  if (early && blockIdx.x == 0) pdl_wait();
 }
 
 template <int HD>
-int launch_warp(const PaArgs& a, int prefix_ctas, int own_ctas, cudaStream_t s) {
+int launch_warp(const PaArgs& a, int prefix_ctas, int own_ctas, bool early, cudaStream_t s) {
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(attn_warp_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -531,13 +537,13 @@ int launch_warp(const PaArgs& a, int prefix_ctas, int own_ctas, cudaStream_t s) 
     attr = true;
   }
   return launch_pdl(attn_warp_kernel<HD>, dim3(static_cast<unsigned>(prefix_ctas) + own_ctas), dim3(32),
-                    sizeof(WarpShared<HD>), s, a, prefix_ctas) == cudaSuccess
+                    sizeof(WarpShared<HD>), s, a, prefix_ctas, early ? 1 : 0) == cudaSuccess
              ? 0
              : SB_OPERR_LAUNCH;
 }
 
 template <int HD>
-int launch(const PaArgs& a, int prefix_ctas, int own_ctas, cudaStream_t s) {
+int launch(const PaArgs& a, int prefix_ctas, int own_ctas, bool early, cudaStream_t s) {
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(attn_mma_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -546,23 +552,23 @@ int launch(const PaArgs& a, int prefix_ctas, int own_ctas, cudaStream_t s) {
     attr = true;
   }
   return launch_pdl(attn_mma_kernel<HD>, dim3(static_cast<unsigned>(prefix_ctas) + own_ctas), dim3(kThreads),
-                    sizeof(MmaShared<HD>), s, a, prefix_ctas) == cudaSuccess
+                    sizeof(MmaShared<HD>), s, a, prefix_ctas, early ? 1 : 0) == cudaSuccess
              ? 0
              : SB_OPERR_LAUNCH;
 }
 
 }  // namespace
 
-int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s) {
-  if (hd == 32) return launch<32>(a, prefix_ctas, own_ctas, s);
-  if (hd == 64) return launch<64>(a, prefix_ctas, own_ctas, s);
-  return launch<128>(a, prefix_ctas, own_ctas, s);
+int attn_mma(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s) {
+  if (hd == 32) return launch<32>(a, prefix_ctas, own_ctas, early, s);
+  if (hd == 64) return launch<64>(a, prefix_ctas, own_ctas, early, s);
+  return launch<128>(a, prefix_ctas, own_ctas, early, s);
 }
 
-int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, cudaStream_t s) {
-  if (hd == 32) return launch_warp<32>(a, prefix_ctas, own_ctas, s);
-  if (hd == 64) return launch_warp<64>(a, prefix_ctas, own_ctas, s);
-  return launch_warp<128>(a, prefix_ctas, own_ctas, s);
+int attn_warp(const PaArgs& a, int hd, int prefix_ctas, int own_ctas, bool early, cudaStream_t s) {
+  if (hd == 32) return launch_warp<32>(a, prefix_ctas, own_ctas, early, s);
+  if (hd == 64) return launch_warp<64>(a, prefix_ctas, own_ctas, early, s);
+  return launch_warp<128>(a, prefix_ctas, own_ctas, early, s);
 }
 
 }  // namespace sb

@@ -7,7 +7,8 @@
 // exponentials at 16 a cycle, 2050 cycles each; measured 3690, because a row
 // tile's softmax (1620) and its products with their commits and waits (2070)
 // follow one another, with the other row tile half a period behind. 512 x 32
-// queries behind 16384 keys, 137 GFLOP: 142 us, 0.60 of the measured bf16 peak.
+// queries behind 16384 keys, 137 GFLOP: 134 us, 0.63 of the measured bf16 peak,
+// with the join (under the power cap, at 1745 MHz, 151).
 // (7 of 16 exponentials as polynomials in FMAs: 4140 cycles.)
 //
 // A block takes up to 256 rows, two tiles of 128, against tiles of 128 keys;
@@ -144,9 +145,7 @@ __device__ __forceinline__ bool special(const PaPiece& w, int care, int j0) {
   return care < j0 + kKeys;
 }
 
-// `early`: launched beside the kernel before it on the stream, whose own
-// predecessors have completed and which writes nothing that this one reads;
-// it is waited for at the end.
+// `early`: see attn_tc's declaration.
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                               const __grid_constant__ CUtensorMap tm_v, PaArgs a,
@@ -681,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     cp_async_wait<0>();
   }
 
-  if (early) pdl_wait();
+  if (early && blockIdx.x == 0) pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == kSoftWarps) {

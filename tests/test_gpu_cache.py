@@ -382,6 +382,36 @@ def test_attention_keeps_unseen_keys_out(kind, cuda):
     assert np.isnan(got[1][:, 5]).all() and np.array_equal(np.delete(got[1], 5, 1), np.delete(clean[1], 5, 1))
 
 
+def test_attention_calls_in_a_row(cuda):
+    """Calls whose kernels overlap, one after the other in one workspace, without a wait between them."""
+    import torch
+    import sheaf_b200 as sb
+
+    a = _Attend("bf16", 32, 8, 64, 16, 4096, [100] * 40, 1, cuda)
+    L, c, b = sb.lib(), _cache((a.k, a.v)), len(a.lens)
+    size = L.sb_op_prefix_attention_workspace_size(c, b, 1, a.hq, a.prefix, a.table.shape[1])
+    ws = torch.empty(size // 4 + 4, device=cuda)
+    pt, t, ln = _i(a.prefix_table, cuda), _i(a.table, cuda), _i(a.lens, cuda)
+    qs = [a.q * (1 - i / 8) for i in range(8)]
+    outs = [torch.empty_like(a.out) for _ in range(16)]
+
+    def attend(q, out):
+        assert L.sb_op_prefix_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), None, b, 1, a.hq,
+                                        a.scale, pt.data_ptr(), a.prefix, t.data_ptr(), a.table.shape[1],
+                                        ln.data_ptr(), ws.data_ptr(), size, _stream()) == 0
+
+    for q, out in zip(qs, outs[:8]):
+        attend(q, out)
+        torch.cuda.synchronize()
+    for _ in range(20):
+        for out in outs[8:]:
+            out.zero_()
+        for q, out in zip(qs, outs[8:]):
+            attend(q, out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs[:8], outs[8:]))
+
+
 @pytest.mark.parametrize("kind,seqs,prefix", [("bf16", 3, 20000), ("bf16", 20, 1500), ("bf16", 70, 20000),
                                               ("f32", 3, 20000), ("f32", 70, 20000)])
 def test_attention_keys_at_minus_infinity(kind, seqs, prefix, cuda):
