@@ -222,8 +222,11 @@ __device__ void attend_wide(const PaArgs& a, const PaPiece& w, WideShared<HD>& s
   most = __reduce_max_sync(0xffffffffu, most);
   const int k1 = __syncthreads_or(most > w.k0) ? w.k1 : w.k0;  // shared memory is free, too
 
+  // Where no row sees a key of the piece nothing is copied: only the loop over
+  // the keys waits for copies, and one still in flight behind it would meet
+  // the next piece's in the same places, in no order.
   constexpr int CH = HD / 4;  // vectors of a row
-  for (int i = tid; i < kWideRows * CH; i += kThreads) {
+  for (int i = w.k0 < k1 ? tid : kWideRows * CH; i < kWideRows * CH; i += kThreads) {
     const int r = w.row0 + i / CH, c = i % CH * 4;
     const bool in = r < w.rows;
     long at = 0;
@@ -255,7 +258,7 @@ __device__ void attend_wide(const PaArgs& a, const PaPiece& w, WideShared<HD>& s
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[r][c][e] = 0.f;
   }
-  load(0, w.k0);
+  if (w.k0 < k1) load(0, w.k0);
   int stage = 0;
   for (int j0 = w.k0; j0 < k1; j0 += kKeys, stage ^= 1) {
     if (j0 + kKeys < k1) {
