@@ -30,8 +30,10 @@ namespace {
 
 enum : int { kRotNone = SB_ROTARY_NONE, kRotHalves = SB_ROTARY_HALVES, kRotPairs = SB_ROTARY_PAIRS };
 
+// (No more than 16-byte alignment: what the entry point and the dispatch below
+// see to. Eight angles are two vectors.)
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
   T v[VEC];
 };
 

@@ -4,7 +4,7 @@ and tolerances as in test_gpu_cache.py."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_cache import _Attend, _attend64, _check_attention, _f64
+from tests.test_gpu_cache import _Attend, _attend64, _cache, _check_attention, _f64, _i, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,34 @@ def test_f32_attention_beside_many_idle_slots(hq, hkv, hd, prefix, idle, cuda):
     for _ in range(20):
         a()
         assert torch.equal(a.out, first) and torch.equal(a.lse, first_lse)
+
+
+# ---- append: tables at odd places ------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("mode", [1, 2])
+def test_append_with_angles_at_any_vector(kind, mode, cuda):
+    """Tables that start 4 and 8 floats into an allocation give what tables at its start give."""
+    import torch
+    import sheaf_b200 as sb
+
+    hq, hkv, hd, n = 8, 2, 64, 33
+    width, g = (hq + 2 * hkv) * hd, torch.Generator().manual_seed(mode)
+    qkv = torch.randn(n, width, generator=g).to(torch.float32 if kind == "f32" else torch.bfloat16).to(cuda)
+    ang = torch.randn(n, hd // 2, generator=g)
+    table, seq, pos = (_i(x, cuda) for x in (np.arange(3)[None], np.zeros(n), np.arange(n)))
+    want = None
+    for shift in (0, 4, 8):
+        cs = torch.zeros(2, shift + ang.numel(), device=cuda)
+        cs[0, shift:], cs[1, shift:] = ang.cos().flatten().to(cuda), ang.sin().flatten().to(cuda)
+        rows = [cs[i].clone() for i in range(2)]  # allocations of their own
+        k, v = (torch.zeros(3, 16, hkv, hd, device=cuda, dtype=qkv.dtype) for _ in range(2))
+        q = torch.zeros(n, hq * hd, device=cuda, dtype=qkv.dtype)
+        assert sb.lib().sb_op_kv_append(_cache((k, v)), qkv.data_ptr(), width, n, hq, q.data_ptr(), hq * hd,
+                                        seq.data_ptr(), pos.data_ptr(), 0, table.data_ptr(), 1, 3, mode, hd,
+                                        rows[0][shift:].data_ptr(), rows[1][shift:].data_ptr(), n, _stream()) == 0
+        if want is None:
+            want = q, k, v
+            assert q.abs().max() > 0 and k.abs().max() > 0
+        assert all(torch.equal(x, y) for x, y in zip((q, k, v), want))
