@@ -42,6 +42,15 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162flo
 __device__ __forceinline__ void from_f32(float& d, float x) { d = x; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16& d, float x) { d = __float2bfloat16_rn(x); }
 
+// (a, b) turned by (c, n) = (cos, sin). Which product of a sum is rounded first
+// is spelt out, for each type as its vector path always had it, so that a value
+// comes out the same whichever path its alignment leads to.
+template <typename T>
+__device__ __forceinline__ float2 turned(float a, float b, float c, float n) {
+  const float x = fmaf(a, c, -__fmul_rn(b, n));
+  return make_float2(x, sizeof(T) == 4 ? fmaf(a, n, __fmul_rn(b, c)) : fmaf(b, c, __fmul_rn(a, n)));
+}
+
 template <typename T>
 struct AppendArgs {
   T* k;
@@ -81,15 +90,15 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
   // element offsets of the unit's two vectors within a head
   const int half = a.rot / 2;
   int e0, e1;
-  bool turned = false;
+  bool turns = false;
   if (MODE == kRotHalves && u < half / VEC) {
     e0 = u * VEC;
     e1 = e0 + half;
-    turned = true;
+    turns = true;
   } else {
     e0 = 2 * u * VEC;
     e1 = e0 + VEC;
-    if (MODE == kRotPairs) turned = e0 < a.rot;
+    if (MODE == kRotPairs) turns = e0 < a.rot;
   }
 
   P x[HPT][2];
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
     const float* ct = a.cos + static_cast<long>(p) * half;
     const float* st = a.sin + static_cast<long>(p) * half;
     if (MODE == kRotHalves || VEC == 1) {
-      if (turned) {
+      if (turns) {
         const int j = MODE == kRotHalves ? e0 : e0 / 2;
         const Pack<float, VEC> c = *reinterpret_cast<const Pack<float, VEC>*>(ct + j);
         const Pack<float, VEC> n = *reinterpret_cast<const Pack<float, VEC>*>(st + j);
@@ -130,9 +139,9 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
           if (h0 + i < a.hq + a.hkv)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-              const float f = to_f32(x[i][0].v[e]), g = to_f32(x[i][1].v[e]);
-              from_f32(x[i][0].v[e], f * c.v[e] - g * n.v[e]);
-              from_f32(x[i][1].v[e], g * c.v[e] + f * n.v[e]);
+              const float2 y = turned<T>(to_f32(x[i][0].v[e]), to_f32(x[i][1].v[e]), c.v[e], n.v[e]);
+              from_f32(x[i][0].v[e], y.x);
+              from_f32(x[i][1].v[e], y.y);
             }
       }
     } else {
@@ -148,9 +157,9 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
           if (h0 + i < a.hq + a.hkv)
 #pragma unroll
             for (int j = 0; j < HV; ++j) {
-              const float f = to_f32(x[i][w].v[2 * j]), g = to_f32(x[i][w].v[(2 * j + 1) % VEC]);
-              from_f32(x[i][w].v[2 * j], f * c.v[j] - g * n.v[j]);
-              from_f32(x[i][w].v[(2 * j + 1) % VEC], g * c.v[j] + f * n.v[j]);
+              const float2 y = turned<T>(to_f32(x[i][w].v[2 * j]), to_f32(x[i][w].v[(2 * j + 1) % VEC]), c.v[j], n.v[j]);
+              from_f32(x[i][w].v[2 * j], y.x);
+              from_f32(x[i][w].v[(2 * j + 1) % VEC], y.y);
             }
       }
     }

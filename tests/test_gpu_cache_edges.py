@@ -48,8 +48,8 @@ def test_f32_attention_beside_many_idle_slots(hq, hkv, hd, prefix, idle, cuda):
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("mode", [1, 2])
-def test_append_with_angles_at_any_vector(kind, mode, cuda):
-    """Tables that start 4 and 8 floats into an allocation give what tables at its start give."""
+def test_append_with_angles_at_any_float(kind, mode, cuda):
+    """Tables that start 4, 1 and 8 floats into an allocation give what tables at its start give."""
     import torch
     import sheaf_b200 as sb
 
@@ -59,7 +59,7 @@ def test_append_with_angles_at_any_vector(kind, mode, cuda):
     ang = torch.randn(n, hd // 2, generator=g)
     table, seq, pos = (_i(x, cuda) for x in (np.arange(3)[None], np.zeros(n), np.arange(n)))
     want = None
-    for shift in (0, 4, 8):
+    for shift in (0, 4, 1, 8):
         cs = torch.zeros(2, shift + ang.numel(), device=cuda)
         cs[0, shift:], cs[1, shift:] = ang.cos().flatten().to(cuda), ang.sin().flatten().to(cuda)
         rows = [cs[i].clone() for i in range(2)]  # allocations of their own
