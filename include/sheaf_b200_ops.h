@@ -189,7 +189,8 @@ SB_API int sb_op_random_split(const void* key, int32_t n, void* out, void* strea
  * the rows alone (sheaf/lib/nn.shf:44-50). These serve callers that draw
  * several answers to one prompt inside the context and learn from the answers'
  * log probabilities. Index arguments (sequences, positions, page tables,
- * lengths) are int32 device arrays; strides are in elements. */
+ * lengths) are int32 device arrays; strides are in elements. A pointer that is
+ * not on whole values of its type returns SB_OPERR_ARGS. */
 
 /* One layer's paged key / value cache: row r of head h of page p starts at
  * element p * page_stride + r * row_stride + h * head_stride of `k` and `v`.

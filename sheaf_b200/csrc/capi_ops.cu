@@ -38,6 +38,12 @@ static bool fill_matmul_desc(GemmDesc& d, uint32_t elem, const void* a, int64_t 
   return true;
 }
 
+// Whether all are pointers to whole 4-byte values (NULL is).
+template <typename... P>
+static bool on_words(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % 4 == 0) && ...);
+}
+
 }  // namespace sb
 
 extern "C" {
@@ -222,6 +228,11 @@ int sb_op_global_norm(uint32_t elem, int32_t n_leaves, const int64_t* counts, co
 
 static bool fits(int64_t v) { return v > -(int64_t{1} << 40) && v < (int64_t{1} << 40); }
 
+// Whether `p` is a pointer to whole values of the element type.
+static bool on_values(const void* p, uint32_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % (elem == SB_ELEM_F32 ? 4 : 2) == 0;
+}
+
 // A usable cache description: strides that keep every 16-byte vector aligned
 // (rows of a head never overlap a neighbour's by less than head_dim).
 static int check_cache(const sb_kv_cache* c) {
@@ -254,6 +265,9 @@ int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld, int32
     if (rot_dim <= 0 || rot_dim % 2 || rot_dim > cache->head_dim || n_pos <= 0 || !cos_table || !sin_table)
       return SB_OPERR_ARGS;
   }
+  if (!on_values(qkv, cache->elem) || !sb::on_words(seq, pos, pages)) return SB_OPERR_ARGS;
+  if (h_q > 0 && !on_values(q_out, cache->elem)) return SB_OPERR_ARGS;
+  if (rotary != SB_ROTARY_NONE && !sb::on_words(cos_table, sin_table)) return SB_OPERR_ARGS;
   sb::AppendDesc d;
   d.cache = *cache;
   d.qkv = qkv;
@@ -313,6 +327,7 @@ int sb_op_prefix_attention(const sb_kv_cache* cache, const void* q, int64_t ldq,
   const int64_t width = static_cast<int64_t>(h_q) * cache->head_dim;
   if (!q || !out || !lens || !fits(ldq) || !fits(ldo) || ldq < width || ldo < width) return SB_OPERR_ARGS;
   if ((prefix_len > 0 && !prefix_pages) || (max_pages > 0 && !pages)) return SB_OPERR_ARGS;
+  if (!sb::on_words(lse, prefix_pages, pages, lens)) return SB_OPERR_ARGS;
   const int64_t vec = cache->elem == SB_ELEM_F32 ? 4 : 8;
   if (ldq % vec || ldo % vec || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
     return SB_OPERR_TMA;
@@ -332,11 +347,6 @@ int sb_op_prefix_attention(const sb_kv_cache* cache, const void* q, int64_t ldq,
                               sb::device_error_word());
 }
 
-// Whether `p` is a pointer to whole values of the element type.
-static bool on_values(const void* p, uint32_t elem) {
-  return reinterpret_cast<uintptr_t>(p) % (elem == SB_ELEM_F32 ? 4 : 2) == 0;
-}
-
 int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v, const void* targets,
                          float temperature, void* logp, void* entropy, void* lse, int32_t k, void* top_ids,
                          void* top_logp, void* stream) {
@@ -345,6 +355,7 @@ int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, int32_t 
   if (!(temperature >= 1e-6f && temperature <= 1e6f)) return SB_OPERR_ARGS;
   if (rows == 0) return 0;
   if (!logits || !on_values(logits, elem) || (logp && !targets)) return SB_OPERR_ARGS;
+  if (!sb::on_words(targets, logp, entropy, lse, top_ids, top_logp)) return SB_OPERR_ARGS;
   sb::LogprobsDesc d;
   d.f32 = elem == SB_ELEM_F32;
   d.x = logits;
@@ -370,6 +381,7 @@ int sb_op_token_logprobs_bwd(uint32_t elem, const void* logits, int64_t ld, int3
   if (rows == 0) return 0;
   if (!logits || !dlogits || !lse || !on_values(logits, elem) || !on_values(dlogits, elem)) return SB_OPERR_ARGS;
   if ((dlogp && !targets) || (dentropy && !entropy)) return SB_OPERR_ARGS;
+  if (!sb::on_words(targets, lse, entropy, dlogp, dentropy)) return SB_OPERR_ARGS;
   if (dlogits == logits && ldd != ld) return SB_OPERR_ARGS;
   sb::LogprobsBwdDesc d;
   d.f32 = elem == SB_ELEM_F32;
