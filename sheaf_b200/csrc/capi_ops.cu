@@ -268,6 +268,7 @@ int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld, int32
   if (!on_values(qkv, cache->elem) || !sb::on_words(seq, pos, pages)) return SB_OPERR_ARGS;
   if (h_q > 0 && !on_values(q_out, cache->elem)) return SB_OPERR_ARGS;
   if (rotary != SB_ROTARY_NONE && !sb::on_words(cos_table, sin_table)) return SB_OPERR_ARGS;
+  if (h_q > 0 && q_out == qkv && ldq != ld) return SB_OPERR_ARGS;  // rows would be read after others are written
   sb::AppendDesc d;
   d.cache = *cache;
   d.qkv = qkv;

@@ -1,5 +1,5 @@
-"""Pointers that are not on whole values
-are refused on the host (nothing is read)."""
+"""Pointers that are not on whole values, and memory that would be read and
+written in two layouts at once, are refused on the host (nothing is read)."""
 import pytest
 
 from tests.test_cache_refusals import ARGS, BF16, F32, P, _append, _attend, _cache, _grad, _score
@@ -15,6 +15,10 @@ def test_append_wants_whole_values(L, change):  # noqa: F811
 def test_append_of_f32_wants_whole_values(L):  # noqa: F811
     for change in (dict(qkv=P + 2, q_out=2 * P), dict(q_out=2 * P + 2)):
         assert _append(L, _cache(elem=F32), **change) == ARGS
+
+
+def test_append_in_place_wants_one_stride(L):  # noqa: F811
+    assert _append(L, qkv=P, q_out=P, ldq=256) == ARGS
 
 
 @pytest.mark.parametrize("change", [dict(lse=P + 2), dict(prefix_pages=P + 2), dict(pages=P + 1), dict(lens=P + 3)])
