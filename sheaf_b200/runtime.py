@@ -225,6 +225,18 @@ class Session:
         if rc:
             raise SheafB200Error(3, f"{what} failed ({rc})")
 
+    @staticmethod
+    def _want(what: str, ok: bool, why: str) -> None:
+        if not ok:
+            raise SheafB200Error(3, f"{what}: {why}")
+
+    def _values(self, what: str, elem: int, count: int, **buffers: "Buffer | None") -> None:
+        """Each buffer given is of type `elem` and holds at least the `count` values that the kernel reads."""
+        for name, b in buffers.items():
+            if b is not None:
+                self._want(what, b.elem == elem and b.nbytes >= count * ELEM_SIZE[elem],
+                           f"{name} has to hold {count} values of type {elem:#x}")
+
     def kv_cache(self, n_pages: int, page_rows: int, n_heads: int, head_dim: int, elem: int = ELEM_BF16) -> "KvPages":
         """One layer's paged keys and values, [n_pages, page_rows, n_heads, head_dim] each."""
         return KvPages(self, n_pages, page_rows, n_heads, head_dim, elem)
@@ -234,9 +246,17 @@ class Session:
         """Appends the keys and values of qkv [n, (h_q + 2 h_kv) hd] at positions pos [n] of sequences seq [n] (pages
         [n_seqs, max_pages] from position base on; i32) and returns the queries [n, h_q hd], rotated as the keys are
         (rotary 1: halves, 2: pairs; cos, sin f32 [n_pos, rot_dim / 2])."""
-        n, width = qkv.shape
         c = cache.desc
+        self._want("kv_append", len(qkv.shape) == 2 and qkv.elem == c.elem and qkv.shape[1] % c.head_dim == 0
+                   and qkv.shape[1] >= 2 * c.n_heads * c.head_dim, "qkv has to be rows of heads in the cache's type")
+        n, width = qkv.shape
         h_q = width // c.head_dim - 2 * c.n_heads
+        self._values("kv_append", ELEM_I32, n, seq=seq, pos=pos)
+        self._want("kv_append", len(pages.shape) == 2 and pages.elem == ELEM_I32, "pages has to be rows of i32")
+        if rotary:
+            self._want("kv_append", cos is not None and sin is not None and len(cos.shape) == 2,
+                       "a rotation has to have rows of cos and sin")
+            self._values("kv_append", ELEM_F32, cos.shape[0] * cos.shape[1], cos=cos, sin=sin)
         q = self.empty((n, h_q * c.head_dim), qkv.elem)
         n_pos, rot = (cos.shape[0], 2 * cos.shape[1]) if rotary else (0, 0)
         self._op("kv_append", lib().sb_op_kv_append(
@@ -251,8 +271,15 @@ class Session:
         """Attention of q [b tq, h_q hd] (b = the entries of lens, i32) to the prefix_len keys that all sequences share
         and each one's own lens[s] keys; returns the output and the log-sum-exp [b tq, h_q] (f32)."""
         c = cache.desc
+        self._want("prefix_attention", len(q.shape) == 2 and q.elem == c.elem and q.shape[1] % c.head_dim == 0,
+                   "q has to be rows of heads in the cache's type")
+        self._want("prefix_attention", len(lens.shape) == 1 and lens.elem == ELEM_I32, "lens has to be i32")
         rows, width = q.shape
         b = lens.shape[0]
+        self._want("prefix_attention", rows % b == 0 if b else rows == 0, "each sequence has to have as many rows")
+        self._want("prefix_attention", pages is None or (len(pages.shape) == 2 and pages.elem == ELEM_I32
+                                                         and pages.shape[0] >= b), "pages has to be a row of i32 each")
+        self._values("prefix_attention", ELEM_I32, -(-prefix_len // c.page_rows), prefix_pages=prefix_pages)
         h_q, max_pages = width // c.head_dim, pages.shape[1] if pages is not None else 0
         out, lse = self.empty((rows, width), q.elem), self.empty((rows, h_q), ELEM_F32)
         shape = (c, b, rows // b if b else 0, h_q, prefix_len, max_pages)
@@ -269,7 +296,9 @@ class Session:
                        k: int = 0) -> dict[str, "Buffer"]:
         """Scores the first v columns of logits [rows, ld] at a temperature: "entropy", "lse" [rows], with targets (f32
         ids) their "logp", with k the likeliest tokens "top_ids" (i32) and "top_logp" [rows, k]."""
+        self._want("token_logprobs", len(logits.shape) == 2, "logits have to be rows")
         rows, ld = logits.shape
+        self._values("token_logprobs", ELEM_F32, rows, targets=targets)
         out = {name: self.empty((rows,), ELEM_F32) for name in ("entropy", "lse")}
         if targets is not None:
             out["logp"] = self.empty((rows,), ELEM_F32)
@@ -287,7 +316,10 @@ class Session:
                            temperature: float = 1.0) -> "Buffer":
         """Gradient [rows, ld] of sum(dlogp logp) + sum(dentropy entropy) in the logits, from token_logprobs's scores;
         columns from v on are not written."""
+        self._want("token_logprobs_vjp", len(logits.shape) == 2, "logits have to be rows")
         rows, ld = logits.shape
+        self._values("token_logprobs_vjp", ELEM_F32, rows, targets=targets, dlogp=dlogp, dentropy=dentropy,
+                     lse=scores["lse"], entropy=scores["entropy"])
         dx = self.empty((rows, ld), logits.elem)
         ptr = lambda b: b.device_ptr if b is not None else None  # noqa: E731
         self._op("token_logprobs_vjp", lib().sb_op_token_logprobs_bwd(
