@@ -167,10 +167,11 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& 
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     const long at = row[r].token * a.hq + row[r].h;
     if (a.direct) {
-      const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      // (a row of zeros where nothing counts: o may hold 0 * inf)
+      const float f = sum > 0.f ? 1.f / sum : sum;
       T* out = static_cast<T*>(a.out) + row[r].token * a.ldo + static_cast<long>(row[r].h) * HD + lane * C;
 #pragma unroll
-      for (int c = 0; c < C; ++c) out[c] = static_cast<T>(o[r][c] * f);
+      for (int c = 0; c < C; ++c) out[c] = sum == 0.f ? T(0.f) : static_cast<T>(o[r][c] * f);
       if (a.lse && lane == 0) a.lse[at] = m[r] + logf(sum);
     } else {
       const long slot = static_cast<long>(w.part) * a.b * a.tq * a.hq + at;
@@ -344,12 +345,14 @@ __device__ void attend_wide(const PaArgs& a, const PaPiece& w, WideShared<HD>& s
     if (w.row0 + warp * 16 + rg * 4 + r >= w.rows) continue;
     const long at = row[r].token * a.hq + row[r].h;
     if (a.direct) {
-      const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      // (a row of zeros where nothing counts: o may hold 0 * inf)
+      const float f = sum > 0.f ? 1.f / sum : sum;
       float* out = static_cast<float*>(a.out) + row[r].token * a.ldo + static_cast<long>(row[r].h) * HD + kg * 4;
 #pragma unroll
       for (int c = 0; c < Q; ++c)
         *reinterpret_cast<float4*>(out + c * 32) =
-            make_float4(o[r][c][0] * f, o[r][c][1] * f, o[r][c][2] * f, o[r][c][3] * f);
+            sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                       : make_float4(o[r][c][0] * f, o[r][c][1] * f, o[r][c][2] * f, o[r][c][3] * f);
       if (a.lse && kg == 0) a.lse[at] = m[r] + logf(sum);
     } else {
       const long slot = static_cast<long>(w.part) * a.b * a.tq * a.hq + at;

@@ -505,11 +505,13 @@ __global__ void __launch_bounds__(32) attn_warp_kernel(PaArgs a, int prefix_ctas
           for (int e = 0; e < 2; ++e) rows.o[n][2 * r + e] += taken_out<HD>(sh.bad, n * 8 + t4 * 2 + e, rows.seen[r]);
       }
       if (a.direct) {
-        const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        // (a row of zeros where nothing counts: o may hold 0 * inf)
+        const float f = l > 0.f ? 1.f / l : l;
         bf* out = static_cast<bf*>(a.out) + x.token * a.ldo + static_cast<long>(x.h) * HD + t4 * 2;
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n)
-          *reinterpret_cast<uint32_t*>(out + n * 8) = pack_bf16x2(rows.o[n][2 * r] * f, rows.o[n][2 * r + 1] * f);
+          *reinterpret_cast<uint32_t*>(out + n * 8) =
+              l == 0.f ? 0u : pack_bf16x2(rows.o[n][2 * r] * f, rows.o[n][2 * r + 1] * f);
         if (a.lse && t4 == 0) a.lse[at] = nat + logf(l);
       } else {
         const long slot = static_cast<long>(w.part) * a.b * a.tq * a.hq + at;

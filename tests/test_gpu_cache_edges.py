@@ -72,3 +72,33 @@ def test_append_with_angles_at_any_float(kind, mode, cuda):
             want = q, k, v
             assert q.abs().max() > 0 and k.abs().max() > 0
         assert all(torch.equal(x, y) for x, y in zip((q, k, v), want))
+
+
+# ---- attention: rows that are zero whatever the cache holds ------------------------
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd,prefix", [(2, 2, 64, 40), (2, 2, 64, 20), (8, 1, 128, 30), (1, 1, 32, 64),
+                                              (8, 1, 64, 64), (8, 1, 32, 32), (80, 1, 64, 64)])
+def test_idle_rows_stay_zero_beside_infinite_values(kind, hq, hkv, hd, prefix, cuda):
+    """Nothing but a short prefix, one part: idle slots share a tile of rows with slots that see an infinite value."""
+    a = _Attend(kind, hq, hkv, hd, 16, prefix, [0, -1, 0, -1, 0], 1, cuda)
+    assert a.table.shape[1] == 0
+    for bad in (float("inf"), float("nan"), float("-inf")):
+        a.v[int(a.prefix_table[0]), 3, :, 7] = bad
+        got, lse = a()
+        idle = a.lens < 0
+        assert (got[idle] == 0).all() and np.isneginf(lse[idle]).all()
+        assert not np.isfinite(got[~idle][..., 7]).any() and np.isfinite(np.delete(got[~idle], 7, 2)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("slots", [3, 9, 80])
+def test_rows_without_a_finite_score_are_zero(kind, slots, cuda):
+    """All scores are -inf, and a value that the rows see is infinite."""
+    a = _Attend(kind, 2, 2, 64, 16, 30, [0] * slots, 1, cuda)
+    a.q[..., ::64] = 1.0
+    a.k[..., 0] = float("-inf")
+    a.v[int(a.prefix_table[0]), 5, :, 9] = float("inf")
+    got, lse = a()
+    assert (got == 0).all() and np.isneginf(lse).all()
