@@ -114,9 +114,10 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& 
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
         const float mn = fmaxf(m[r], t);
-        // a row that has seen no key keeps m = -inf, l = 0
+        // a row that has seen no key keeps m = -inf, l = 0; NaN scores, which
+        // the maximum passes over, go to p whatever it is
         const float f = mn == -INFINITY ? 1.f : expf(m[r] - mn);
-        p[r] = mn == -INFINITY ? 0.f : expf(s[r] - mn);
+        p[r] = expf(s[r] - (mn == -INFINITY ? 0.f : mn));
         l[r] = l[r] * f + p[r];
         m[r] = mn;
 #pragma unroll
@@ -296,10 +297,11 @@ __device__ void attend_wide(const PaArgs& a, const PaPiece& w, WideShared<HD>& s
         for (int x = 4; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
         const float mn = fmaxf(m[r], t);
         const float f = mn == -INFINITY ? 1.f : expf(m[r] - mn);
+        const float sub = mn == -INFINITY ? 0.f : mn;  // a NaN score stays one
         l[r] *= f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[r][i] = mn == -INFINITY ? 0.f : expf(s[r][i] - mn);
+          s[r][i] = expf(s[r][i] - sub);
           l[r] += s[r][i];
         }
         m[r] = mn;

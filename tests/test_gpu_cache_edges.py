@@ -102,3 +102,33 @@ def test_rows_without_a_finite_score_are_zero(kind, slots, cuda):
     a.v[int(a.prefix_table[0]), 5, :, 9] = float("inf")
     got, lse = a()
     assert (got == 0).all() and np.isneginf(lse).all()
+
+
+# ---- attention: NaN is not hidden ----------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd,prefix,lens", [(2, 2, 64, 40, [3, 2]), (8, 2, 128, 300, [5] * 9),
+                                                   (4, 4, 64, 2000, [40] * 80)])
+def test_nan_queries_and_keys_show(kind, hq, hkv, hd, prefix, lens, cuda):
+    """A NaN query's row is NaN and no other; so is every row that sees a NaN key, the first of all or its only one."""
+    a = _Attend(kind, hq, hkv, hd, 16, prefix, lens, 1, cuda)
+    clean, clean_lse = a()
+    q = a.q.clone()
+    a.q[1, 5] = float("nan")            # head 0 of sequence 1
+    got, lse = a()
+    assert np.isnan(got[1, 0]).all() and np.isnan(lse[1, 0])
+    got[1, 0], lse[1, 0] = clean[1, 0], clean_lse[1, 0]
+    assert np.array_equal(got, clean) and np.array_equal(lse, clean_lse)
+    a.q.copy_(q)
+    a.k[int(a.table[0][0]), 0] = float("nan")  # the first of sequence 0's own keys
+    got, lse = a()
+    assert np.isnan(got[0]).all() and np.isnan(lse[0]).all()
+    assert np.array_equal(got[1:], clean[1:]) and np.array_equal(lse[1:], clean_lse[1:])
+    a.k[int(a.prefix_table[0])] = float("nan")  # the first keys of all
+    got, lse = a()
+    assert np.isnan(got).all() and np.isnan(lse).all()
+    a.prefix, a.lens = 0, np.ones_like(a.lens)   # its own first key alone
+    got, lse = a()
+    assert np.isnan(got[0]).all() and np.isnan(lse[0]).all()
+    assert np.isfinite(got[1:]).all() and np.isfinite(lse[1:]).all()
