@@ -9,8 +9,9 @@
 //   lse = ln2 (R + log2 S),   H = ln2 (log2 S - W / S)
 // y - R is one fused multiply-add with a single rounding, and references differ
 // by whole numbers, so joining two threads' sums scales by exact powers of two.
-// Logits below -1e29 count as -inf there; a row with nothing else is taken
-// again by differences of the logits themselves.
+// Logits below -1e29 count as -inf there. A row with nothing else, or whose
+// reference passes 2^22, where floats thin out to whole numbers and S could end
+// up far below 1, is taken again by differences of the logits themselves.
 //
 // The k best (larger value first, then lower index) come from the same pass:
 // each thread remembers its largest 16-byte vector. The k-th largest of 64
@@ -142,12 +143,22 @@ __device__ __forceinline__ Stats merge(Stats a, Stats b) {
   raise(b, r);
   return {r, a.s + b.s, a.w + b.w};
 }
+// A reference for x, whose y passes a's: ceil(x c), and where that product's
+// rounding says too little by whole numbers (from 2^24 on; an exponential could
+// pass the largest float from 2^32 on), what the rounding left, rounded up.
+__device__ __forceinline__ void raise_for(Stats& a, float x, float c) {
+  float r = ceilf(x * c);
+  const float over = fmaf(x, c, -r);
+  if (over > 0.5f) r = __fadd_ru(r, over);
+  raise(a, r);
+}
 // One value of at least -1e30, or NaN, under a reference >= x c.
 __device__ __forceinline__ void take(Stats& a, float x, float c) {
   const float y = fmaf(x, c, -a.r), e = ex2_approx(y);
   a.s += e;
   a.w = fmaf(e, y, a.w);
 }
+constexpr float kFar = 4194304.f;  // 2^22: up to here R is a whole number within 2 of the largest y
 constexpr float kLow = -1e29f;
 
 template <int W>
@@ -248,7 +259,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 32, W == 1 ? 6 : 40 / W) lo
 #pragma unroll
     for (int j = 1; j < U; ++j) top = max_nan(top, hi[j]);
     if (top < kLow) continue;
-    if (top * c > st.r) raise(st, ceilf(top * c));
+    if (fmaf(top, c, -st.r) > 0.f) raise_for(st, top, c);
     const float2 r2 = make_float2(-st.r, -st.r), c2 = make_float2(c, c);
     float2 s2 = make_float2(st.s, 0.f), w2 = make_float2(st.w, 0.f);
 #pragma unroll
@@ -271,7 +282,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 32, W == 1 ? 6 : 40 / W) lo
   if (tid < loose) {
     const float f = Elem<T>::get(x + loose_at(tid));
     if (!(f < kLow)) {
-      if (f * c > st.r) raise(st, ceilf(f * c));
+      if (fmaf(f, c, -st.r) > 0.f) raise_for(st, f, c);
       take(st, f, c);
     }
   }
@@ -446,10 +457,10 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 32, W == 1 ? 6 : 40 / W) lo
     all = sh.all;
   }
 
-  // Nothing above -1e29: the sums again, by differences to the largest logit,
-  // over the whole row.
+  // Nothing above -1e29, or a reference too far out: the sums again, by
+  // differences to the largest logit, over the whole row.
   float ref = 0.f;  // what is taken off the logits first
-  const bool low = all.s == 0.f;
+  const bool low = all.s == 0.f || (all.s == all.s && fabsf(all.r) > kFar);
   if (low) {
     float m = kNegInf;
     for (int i = tid; i < a.v; i += NT) m = fmaxf(m, Elem<T>::get(x + i));
@@ -488,10 +499,11 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 32, W == 1 ? 6 : 40 / W) lo
   const auto logp_of = [&](float f) {
     if (all.s != all.s) return all.s;
     if (f == kNegInf) return kNegInf;
-    return (fmaf(low ? f - ref : f, c, -all.r) - log_s) * kLn2;
+    if (low) return fmaf(f - ref, a.inv_t, -log_s * kLn2);  // in log2 units it might pass the largest float
+    return (fmaf(f, c, -all.r) - log_s) * kLn2;
   };
   if (tid == 0) {
-    // ref / temperature and r + log2 S, the first 0 unless the row is low
+    // ref / temperature and r + log2 S, the first 0 unless the row was taken again
     if (a.lse) a.lse[row] = all.s != all.s ? all.s : (none ? kNegInf : fmaf(ref, a.inv_t, (all.r + log_s) * kLn2));
     if (a.entropy) a.entropy[row] = none ? 0.f : (log_s - all.w / all.s) * kLn2;
     if (a.logp) {

@@ -4,7 +4,7 @@ and tolerances as in test_gpu_cache.py."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_cache import _Attend, _attend64, _cache, _check_attention, _f64, _i, _stream
+from tests.test_gpu_cache import ELEM, U, _Attend, _attend64, _cache, _check_attention, _f64, _i, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,58 @@ def test_nan_queries_and_keys_show(kind, hq, hkv, hd, prefix, lens, cuda):
     got, lse = a()
     assert np.isnan(got[0]).all() and np.isnan(lse[0]).all()
     assert np.isfinite(got[1:]).all() and np.isfinite(lse[1:]).all()
+
+
+# ---- log probabilities far from zero ----------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,v,k", [(40, 40, 8), (40, 1031, 20), (40, 5000, 8), (400, 9001, 5), (400, 40000, 0)])
+@pytest.mark.parametrize("temperature", [1e-6, 1.0, 1e6])
+def test_logprobs_of_large_logits(kind, rows, v, k, temperature, cuda):
+    """Logits far from zero, whose ratio to the temperature leaves no bits behind its point in float32."""
+    import torch
+    import sheaf_b200 as sb
+
+    rng = np.random.default_rng(v)
+    at = np.array([3e3, 2e4, 1e6, 8657043456.0, 1e10, -1e10, 1e20, -1e20, 1e28, -3e37, 3e37, -7e3, 0.0, 4.2e6, 8.5e6,
+                   -8.5e6, 1.7e7, 2.0 ** 31, -2.0 ** 33, 3003.0])
+    s = at[np.arange(rows) % len(at)][:, None]
+    x = s + np.abs(s) * 2.0 ** -7 * rng.standard_normal((rows, v)) + rng.standard_normal((rows, v))
+    x[::2, v // 3] = x[::2].max(1)                                   # two equal largest ones
+    x[::3, : v // 2] = -np.inf
+    x[::5] = s[::5]                                                  # all equal
+    xd = torch.from_numpy(x.astype(np.float32)).to(torch.float32 if kind == "f32" else torch.bfloat16).to(cuda)
+    x64 = _f64(xd)
+    t = np.where(np.arange(rows) % 2 == 0, x64.argmax(1), rng.integers(0, v, rows)).astype(np.float32)
+    td = torch.from_numpy(t).to(cuda)
+    logp, ent, lse, alt = (torch.full(n, 9.0, device=cuda) for n in ((rows,), (rows,), (rows,), (rows, max(k, 1))))
+    ids = torch.full((rows, max(k, 1)), -9, device=cuda, dtype=torch.int32)
+    assert sb.lib().sb_op_token_logprobs(ELEM[kind], xd.data_ptr(), v, rows, v, td.data_ptr(), temperature,
+                                         logp.data_ptr(), ent.data_ptr(), lse.data_ptr(), k, ids.data_ptr(),
+                                         alt.data_ptr(), _stream()) == 0
+    big = float(np.finfo(np.float32).max)
+    as_f32 = lambda a: np.where(a > big, np.inf, np.where(a < -big, -np.inf, a))  # noqa: E731
+    z = x64 / float(np.float32(temperature))
+    m = z.max(1, keepdims=True)
+    log_sum = np.log(np.exp(z - m).sum(1, keepdims=True))
+    lp = (z - m) - log_sum
+    with np.errstate(invalid="ignore"):
+        ent64 = -np.where(np.exp(lp) > 0, np.exp(lp) * lp, 0).sum(1)
+    at_t = np.take_along_axis(lp, t.astype(int)[:, None], 1)[:, 0]
+    # the arithmetic's bounds as in test_logprobs: few roundings of each result and, for lse, of the largest z
+    for got, want, size in ((lse, (m + log_sum)[:, 0], np.abs(m[:, 0])), (logp, at_t, np.zeros(rows))):
+        got, want = _f64(got), as_f32(want)
+        assert np.array_equal(np.isinf(got), np.isinf(want)) and not np.isnan(got).any()
+        ok = np.isfinite(want)
+        assert (got[~ok] == want[~ok]).all()
+        w = np.abs(want[ok])
+        assert (np.abs(got[ok] - want[ok]) <= 1e-6 + 256 * U * w.clip(0, 1) + 4 * U * (w + size[ok])).all()
+    assert (np.abs(_f64(ent) - ent64) <= 256 * U * np.maximum(ent64, 0.05)).all()
+    if k:
+        best = np.argsort(-x64, axis=1, kind="stable")[:, :k]
+        assert np.array_equal(ids.cpu().numpy(), best)
+        a64, a = as_f32(np.take_along_axis(lp, best, 1)), _f64(alt)
+        assert np.array_equal(np.isneginf(a), np.isneginf(a64))
+        ok = np.isfinite(a64)
+        assert (np.abs(a[ok] - a64[ok]) <= 1e-6 + 16 * U * (1 + np.abs(a64[ok]))).all()
