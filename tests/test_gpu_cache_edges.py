@@ -187,3 +187,72 @@ def test_logprobs_of_large_logits(kind, rows, v, k, temperature, cuda):
         assert np.array_equal(np.isneginf(a), np.isneginf(a64))
         ok = np.isfinite(a64)
         assert (np.abs(a[ok] - a64[ok]) <= 1e-6 + 16 * U * (1 + np.abs(a64[ok]))).all()
+
+
+# ---- attention: infinite and NaN values in every kernel -----------------------------------
+
+BAD_VALUES = [
+    # kind, hq, hkv, hd, page, prefix, lens, tq: what the rows see ends inside tiles
+    ("bf16", 6, 2, 64, 16, 200, [20, 33, -1, 7], 1),           # a warp: 12 rows behind the prefix, 3 own ones
+    ("bf16", 4, 4, 128, 16, 200, [20] * 7 + [9], 3),           # 4 warps, 128 values: 24 rows
+    ("bf16", 2, 2, 128, 12, 300, [61, 7] * 9, 3),              # 4 warps, pages of 12: 54 rows
+    ("bf16", 1, 1, 64, 20, 500, [90, 41, 120], 40),            # 4 warps, pages of 20: 120 rows, several row tiles
+    ("bf16", 4, 1, 64, 16, 600, [130, 5, -1, 64], 30),         # tcgen05: prefix of 480 rows, own 120
+    ("bf16", 4, 4, 32, 24, 2000, [40, 3] * 50, 1),             # tcgen05: 100 rows, key tiles dealt out
+    ("bf16", 4, 2, 128, 64, 5000, [129, 200, 70], 40),         # tcgen05: 240 rows, own 80
+    ("bf16", 8, 1, 64, 8, 0, [1000, 257], 37),                 # own keys alone, 296 rows
+    ("bf16", 1, 1, 128, 16, 13000, [500], 24),                 # tcgen05: 24 rows, key tiles dealt out; own on 4 warps
+    ("f32", 6, 2, 64, 16, 200, [20, 33, -1, 7], 1),
+    ("f32", 4, 4, 128, 16, 300, [20] * 7 + [9], 3),
+    ("f32", 4, 1, 64, 24, 600, [130, 5, -1, 64], 30),
+]
+
+
+@pytest.mark.parametrize("kind,hq,hkv,hd,page,prefix,lens,tq", BAD_VALUES)
+def test_attention_infinite_values_reach_those_that_see_them(kind, hq, hkv, hd, page, prefix, lens, tq, cuda):
+    """Infinities and NaN in values: first in keys that only some queries see, then behind every query's last key, then
+    in the shared prefix. A column of a row is then NaN or infinite where the row sees such a key, and otherwise bit for
+    bit what it was; and the call repeats itself."""
+    import torch
+
+    a = _Attend(kind, hq, hkv, hd, page, prefix, lens, tq, cuda, capacity=max(lens) + page)
+    lens = np.array(lens)
+    clean, clean_lse = a()
+    group = hq // hkv
+    hit = np.zeros(clean.shape, bool)
+
+    def spoil(table, j, head, col, x, rows):
+        a.v[int(table[j // page]), j % page, head, col] = x
+        hit[rows, head * group:(head + 1) * group, col] = True
+
+    def check():
+        got, lse = a()
+        assert np.array_equal(got[~hit], clean[~hit]) and not np.isfinite(got[hit]).any()
+        assert np.array_equal(lse, clean_lse)
+        first = a.out.clone()
+        for _ in range(3):
+            a()
+            assert torch.equal(a.out.view(torch.uint8), first.view(torch.uint8))
+
+    for s in np.nonzero(lens >= 0)[0]:
+        n = lens[s]
+        # behind the end: nobody sees it
+        for j in range(n, min(n + 3, a.table.shape[1] * page)):
+            spoil(a.table[s], j, hkv - 1, j % hd, float("nan"), [])
+        # the last key (the last query's own) and an earlier one among the queries' own
+        for j, col, x in ((n - 1, 1, float("inf")), (n - tq // 2 - 1, 2, float("nan")), (n - tq, 3, float("-inf")),
+                          (n // 3, 4, float("inf"))):
+            if 0 <= j < n:
+                spoil(a.table[s], j, s % hkv, (col * 7 + s) % hd, x,
+                      [s * tq + t for t in range(tq) if n - tq + t >= j])
+    check()
+    if prefix:
+        # behind the prefix's end, and inside, where short sequences with several queries stop before it
+        for j in range(prefix, min(prefix + 2, len(a.prefix_table) * page)):
+            a.v[int(a.prefix_table[j // page]), j % page, 0, 5] = float("inf")
+        check()
+        for j, col, x in ((prefix - 1, 11, float("nan")), (prefix - max(tq - 2, 1), 12, float("inf")),
+                          (prefix // 2, 13, float("-inf"))):
+            spoil(a.prefix_table, j, 0, col, x,
+                  [s * tq + t for s in np.nonzero(lens >= 0)[0] for t in range(tq) if prefix + lens[s] - tq + t >= j])
+            check()
