@@ -64,8 +64,8 @@ struct Tc {
   static constexpr int kK = kQ + 2 * kTile;
   static constexpr int kV = kK + kStages * kTile;
   static constexpr int kOut = kV + kStages * kTile;
-  static constexpr int kBad = kOut + kSoftWarps * kStageOut;  // int [3][HD]
-  static constexpr int kFound = kBad + 3 * HD * 4;  // int: the piece that kBad is about, plus one
+  static constexpr int kBad = kOut + kSoftWarps * kStageOut;  // int [2][3][HD]
+  static constexpr int kFound = kBad + 2 * 3 * HD * 4;  // int: the piece that kBad is about, plus one
   static constexpr int kDone = kFound + 16;         // int [softmax warps]: pieces finished
   static constexpr int kBars = kDone + 4 * kSoftWarps;
   static constexpr int kNumBars = 2 + 5 * kStages + 6;
@@ -96,7 +96,9 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 }
 
 // What the values taken out of column c add to a row that sees `seen` keys
-// (bad: first key with NaN, +inf, -inf in a column).
+// (bad: first key with NaN, +inf, -inf in a column; where key tiles are dealt
+// out to the two softmax groups, among a group's own ones: a value counts in
+// the part of its tile, and nothing is added while a group reads).
 template <int HD>
 __device__ __forceinline__ float taken_out(const int* bad, int c, int seen) {
   const bool up = bad[HD + c] < seen, down = bad[2 * HD + c] < seen;
@@ -292,11 +294,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                   break;
                 }
               }
-              for (int i = lane; i < 3 * HD; i += 32) bad[i] = 0x7fffffff;
+              for (int i = lane; i < 2 * 3 * HD; i += 32) bad[i] = 0x7fffffff;
               __syncwarp();
               if (lane == 0) *found = piece + 1;
               __syncwarp();
             }
+            if (deal) bad += ((j0 - w.k0) / kKeys & 1) * 3 * HD;
             for (int i = lane; i < rows * CH; i += 32) {
               const int r = i / CH, c = i % CH;
               uint4* p = reinterpret_cast<uint4*>(tile + chunk_at(r, c));
@@ -622,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       // rows leave through shared memory, 64 bytes of 8 rows a store
       if (mine.tiles > 0 || a.direct) {
         const bool some = mine.tiles > 0 && *reinterpret_cast<volatile const int*>(sm + L::kFound) == piece + 1;
-        const int* bad = reinterpret_cast<const int*>(sm + L::kBad);
+        const int* bad = reinterpret_cast<const int*>(sm + L::kBad) + (deal ? x * 3 * HD : 0);
         const long row_at = !mine.in || (!a.direct && l == 0.f) ? -1 : (a.direct ? mine.out_at : part_at * HD);
         const float scale = a.direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
         long their_at[4];

@@ -256,3 +256,22 @@ def test_attention_infinite_values_reach_those_that_see_them(kind, hq, hkv, hd, 
             spoil(a.prefix_table, j, 0, col, x,
                   [s * tq + t for s in np.nonzero(lens >= 0)[0] for t in range(tq) if prefix + lens[s] - tq + t >= j])
             check()
+
+
+@pytest.mark.parametrize("hd,seqs,prefix,key", [(64, 50, 2000, 1990), (128, 50, 2000, 1990), (64, 50, 1900, 1800),
+                                                (32, 50, 2000, 1990)])
+def test_attention_value_counts_once_where_key_tiles_are_dealt(hd, seqs, prefix, key, cuda):
+    """tcgen05, one row tile whose key tiles two groups of warps take in turn: an infinite value belongs to the part of
+    its own tile alone, and stays infinite (not 0 * inf) where that part has all the weight."""
+    a = _Attend("bf16", 4, 4, hd, 16, prefix, [0] * seqs, 2, cuda)  # the first query of each stops a key early
+    q = a.q.view(-1, 4, hd)
+    q[..., 0] = 8.0
+    a.k[..., 0] = 0.0
+    tile = key // 128 * 128
+    for j in range(tile, min(tile + 128, prefix)):
+        a.k[int(a.prefix_table[j // 16]), j % 16, :, 0] = 8.0 * hd ** 0.5   # 64 more than others get
+    a.scale *= 4                                                                # 256
+    a.v[int(a.prefix_table[key // 16]), key % 16, :, 3] = float("inf")
+    for _ in range(10):
+        got, _ = a()
+        assert (got[..., 3] == np.inf).all() and np.isfinite(np.delete(got, 3, 2)).all()
