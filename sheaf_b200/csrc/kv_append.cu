@@ -115,15 +115,15 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs<T> a) {
   if (live && (s >= a.n_seqs || p < a.base || (MODE != kRotNone && p >= a.n_pos) ||
                static_cast<int>(a.page_rows(p - a.base)) >= a.max_pages)) {
     live = false;
-    if (a.err) atomicExch(a.err, kErrIndex);
+    report_index(a.err);
   }
   long row = -1;  // element offset of the token's row in the cache
   if (live) {
     const int own = p - a.base, nth = a.page_rows(own), page = a.pages[static_cast<long>(s) * a.max_pages + nth];
     if (page >= 0 && page < a.n_pages)
       row = page * a.page_stride + static_cast<long>(own - nth * static_cast<int>(a.page_rows.d)) * a.row_stride;
-    else if (a.err)
-      atomicExch(a.err, kErrIndex);
+    else
+      report_index(a.err);
   }
 
   if (MODE != kRotNone && live && h0 < a.hq + a.hkv) {

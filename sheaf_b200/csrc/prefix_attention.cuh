@@ -91,7 +91,7 @@ struct PaPiece {
 __device__ __forceinline__ int seq_len(const PaArgs& a, int s) {
   const int n = a.lens[s];
   if (n > a.capacity) {
-    if (a.err) atomicExch(a.err, kErrIndex);
+    report_index(a.err);
     return a.capacity;
   }
   return n;
@@ -181,7 +181,7 @@ __device__ __forceinline__ PaPiece own_piece(const PaArgs& a, int i) {
 __device__ __forceinline__ int page_of(const PaArgs& a, const int* table, int j) {
   int page = table[a.page_rows(j)];
   if (page < 0 || page >= a.n_pages) {
-    if (a.err) atomicExch(a.err, kErrIndex);
+    report_index(a.err);
     page = 0;
   }
   return page;

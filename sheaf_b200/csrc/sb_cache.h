@@ -13,6 +13,10 @@ namespace sb {
 // Error-word code of an index (page, position) outside what it indexes: the
 // kernel skips the access and records this (sb_op_device_error).
 constexpr int kErrIndex = 2;
+// (It does not take the place of a timeout, which is the graver news.)
+__device__ __forceinline__ void report_index(int* err) {
+  if (err) atomicCAS(err, 0, kErrIndex);
+}
 
 // Division of a non-negative 31-bit number by a fixed d >= 1: n / d =
 // (n * mul) >> 32 >> shift with mul = floor(2^(32 + shift) / d) + 1, 2^shift
