@@ -275,3 +275,23 @@ def test_attention_value_counts_once_where_key_tiles_are_dealt(hd, seqs, prefix,
     for _ in range(10):
         got, _ = a()
         assert (got[..., 3] == np.inf).all() and np.isfinite(np.delete(got, 3, 2)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,tq", [(1, 1, 1), (4, 2, 8), (4, 2, 20), (2, 2, 65), (8, 1, 40)])
+def test_attention_over_an_empty_cache(kind, hq, hkv, tq, cuda):
+    """A cache without pages and nothing to see: zero rows, whichever kernel has as many rows."""
+    import torch
+    import sheaf_b200 as sb
+
+    b, hd = 3, 64
+    c = sb.KvCache(None, None, 16 * hkv * hd, hkv * hd, hd, 0, 16, hkv, hd, ELEM[kind])
+    q = torch.randn(b * tq, hq * hd, device=cuda).to(torch.float32 if kind == "f32" else torch.bfloat16)
+    out, lse = torch.full_like(q, 9.0), torch.full((b * tq, hq), 9.0, device=cuda)
+    lens = _i([0, -1, 0], cuda)
+    size = sb.lib().sb_op_prefix_attention_workspace_size(c, b, tq, hq, 0, 0)
+    ws = torch.full((size // 4 + 4,), float("nan"), device=cuda)
+    assert sb.lib().sb_op_prefix_attention(c, q.data_ptr(), hq * hd, out.data_ptr(), hq * hd, lse.data_ptr(), b, tq, hq,
+                                           0.125, None, 0, None, 0, lens.data_ptr(), ws.data_ptr(), size,
+                                           _stream()) == 0
+    assert (out == 0).all() and torch.isneginf(lse).all()
