@@ -195,6 +195,12 @@ __device__ __forceinline__ const int* table_of(const PaArgs& a, const PaPiece& w
   return w.seq < 0 ? a.prefix_pages : a.pages + static_cast<long>(w.seq) * a.max_pages;
 }
 
+// Whether a reference of exponents in log2 units lies so far out that s sl - ref,
+// fused, may differ by whole numbers from what the reference's own rounding of
+// the product says (beyond 2^24; by hundreds from 2^32 on, which are 0 or
+// infinite weights). Scores are then scaled and rounded before the difference.
+__device__ __forceinline__ bool far_out(float ref) { return ref != -INFINITY && fabsf(ref) > 4194304.f; }
+
 bool cache_map(void* map, const void* base, const PaArgs& a, int hd);
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {

@@ -115,6 +115,7 @@ struct Rows {
   int lo;        // of the warp's rows, for masking
   float o[HD / 8][4];
   float ref[2], l[2];
+  float lim[2];  // scores above it raise the reference; -inf where a row's is far out
 
   __device__ __forceinline__ void start(const PaArgs& a, const PaPiece& w, int row0) {
     const int g = threadIdx.x % 32 / 4, t4 = threadIdx.x % 4;
@@ -136,7 +137,7 @@ struct Rows {
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s][r] = q[s][r + 2] = 0u;
       }
-      ref[r] = -INFINITY;
+      ref[r] = lim[r] = -INFINITY;
       l[r] = 0.f;
     }
     lo = __reduce_min_sync(0xffffffffu, min(seen[0], seen[1]));
@@ -179,7 +180,8 @@ struct Rows {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
       mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * sl;
-    if (__any_sync(0xffffffffu, mx[0] > ref[0] + 8.f || mx[1] > ref[1] + 8.f)) {
+    float by = sl;
+    if (__any_sync(0xffffffffu, mx[0] > lim[0] || mx[1] > lim[1])) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
@@ -194,6 +196,17 @@ struct Rows {
           o[n][2 * r + 1] *= f;
         }
       }
+      const bool far = __any_sync(0xffffffffu, far_out(ref[0]) || far_out(ref[1]));
+      lim[0] = far ? -INFINITY : ref[0] + 8.f;
+      lim[1] = far ? -INFINITY : ref[1] + 8.f;
+      if (far) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[0][e] *= sl;
+          s[1][e] *= sl;
+        }
+        by = 1.f;
+      }
     }
     // p as the sum of two bf16: rounding it to one would add as much error as
     // the output's own rounding, and the second product is free beside the
@@ -204,7 +217,7 @@ struct Rows {
       const float sub = ref[r] == -INFINITY ? 0.f : ref[r];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const float p0 = ex2_approx(fmaf(s[n][2 * r], sl, -sub)), p1 = ex2_approx(fmaf(s[n][2 * r + 1], sl, -sub));
+        const float p0 = ex2_approx(fmaf(s[n][2 * r], by, -sub)), p1 = ex2_approx(fmaf(s[n][2 * r + 1], by, -sub));
         l[r] += p0 + p1;
         const uint32_t h = pack_bf16x2(p0, p1);
         hi[r + 2 * n] = h;

@@ -509,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int least = __reduce_min_sync(0xffffffffu, seen);
       float ref = -INFINITY, l = 0.f;
       bool open = true;  // some row has no reference yet: every score it has seen is -inf
+      bool far = false;  // some row's reference is far out
       for (int j = 0; j < mine.tiles; ++j, ++c) {
         const int j0 = w.k0 + (deal ? 2 * j + x : j) * kKeys;
         if (!wait(&s_full[x], c & 1)) break;
@@ -538,19 +539,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           if (open) {
             if (ref == -INFINITY) ref = mx * sl;
             open = __any_sync(0xffffffffu, ref == -INFINITY && j0 + kKeys < seen);
+            far = __any_sync(0xffffffffu, far_out(ref));
           }
         }
+        float by = sl;
+        if (__builtin_expect(far, 0)) {
+#pragma unroll 1
+          for (int cc = 0; cc < 8; ++cc) {
+            uint32_t u[16];
+            tmem_ld16(tS + cc * 16, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int t = 0; t < 16; ++t) u[t] = __float_as_uint(__uint_as_float(u[t]) * sl);
+            tmem_st16(tS + cc * 16, u);
+          }
+          tmem_wait_st();
+          by = 1.f;
+        }
         uint32_t v[4][32];
-        const float2 sl2 = make_float2(sl, sl);
         float2 sum[2];
-        const auto exps = [&](int cc) {
+        const auto exps = [&](int cc, float by) {
+          const float2 by2 = make_float2(by, by);
           const float sub = ref == -INFINITY ? 0.f : ref;
           const float2 sub2 = make_float2(-sub, -sub);
           uint32_t pk[16];
 #pragma unroll
           for (int t = 0; t < 16; ++t) {
             const float2 y = __ffma2_rn(
-                make_float2(__uint_as_float(v[cc][2 * t]), __uint_as_float(v[cc][2 * t + 1])), sl2, sub2);
+                make_float2(__uint_as_float(v[cc][2 * t]), __uint_as_float(v[cc][2 * t + 1])), by2, sub2);
             const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
             sum[t & 1] = __fadd2_rn(sum[t & 1], p);
             pk[t] = pack_bf16x2(p.x, p.y);
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         for (int cc = 0; cc < 4; ++cc) {
           tmem_wait_ld();
           if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, v[cc + 1]);
-          exps(cc);
+          exps(cc, by);
         }
         float tile_l = total();
         // A NaN is left as it is.
@@ -575,12 +591,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
             for (int t = 0; t < 32; t += 2) {
-              m[0] = fmaxf(m[0], __uint_as_float(v[cc][t]) * sl);
-              m[1] = fmaxf(m[1], __uint_as_float(v[cc][t + 1]) * sl);
+              const float s0 = __uint_as_float(v[cc][t]) * by, s1 = __uint_as_float(v[cc][t + 1]) * by;
+              m[0] = fmaxf(m[0], s0);
+              m[1] = fmaxf(m[1], s1);
+              v[cc][t] = __float_as_uint(s0);
+              v[cc][t + 1] = __float_as_uint(s1);
             }
           const float mx = fmaxf(m[0], m[1]);
           const float f = mx == -INFINITY ? 1.f : ex2_approx(ref - mx);
           ref = mx;
+          far = __any_sync(0xffffffffu, far_out(ref));
           l *= f;
           if (j > 0) {
             if (!wait(&o_full[x], (c - 1) & 1)) break;
@@ -596,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           }
           sum[0] = sum[1] = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) exps(cc);
+          for (int cc = 0; cc < 4; ++cc) exps(cc, 1.f);
           tile_l = total();
         }
         l += tile_l;

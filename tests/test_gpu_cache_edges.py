@@ -4,7 +4,7 @@ and tolerances as in test_gpu_cache.py."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_cache import ELEM, U, _Attend, _attend64, _cache, _check_attention, _f64, _i, _stream
+from tests.test_gpu_cache import ELEM, U, _Attend, _attend64, _cache, _check_attention, _f64, _i, _stream, _t
 
 pytestmark = pytest.mark.gpu
 
@@ -295,3 +295,30 @@ def test_attention_over_an_empty_cache(kind, hq, hkv, tq, cuda):
                                            0.125, None, 0, None, 0, lens.data_ptr(), ws.data_ptr(), size,
                                            _stream()) == 0
     assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+# ---- attention: scores far from zero ----------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd,prefix,lens,tq", [(2, 2, 64, 40, [3, 9], 1), (8, 2, 128, 300, [5] * 9, 1),
+                                                      (4, 4, 64, 2000, [40] * 80, 1), (2, 1, 128, 0, [300, 5], 40)])
+@pytest.mark.parametrize("size", [1e6, 3e9, 1e12, -1e12, 1e30])
+def test_attention_of_large_scores(kind, hq, hkv, hd, prefix, lens, tq, size, cuda):
+    """Scores of one size (a single product of each query, the same with every key): all visible keys weigh the same,
+    or, where a key has none of it, everything or nothing."""
+    a = _Attend(kind, hq, hkv, hd, 16, prefix, lens, tq, cuda)
+    a.q.zero_()
+    a.k.zero_()
+    q = a.q.view(-1, hq, hd)
+    r = np.arange(1, q.shape[0] * hq + 1).reshape(-1, hq)
+    x = np.sqrt(abs(size)) * (1 + (r % 37) / 37)     # of all mantissas
+    q[..., 3] = _t(x, kind, cuda) * float(np.sign(size))
+    a.k[..., 3] = float(np.sqrt(abs(size)))
+    a.scale = 0.7
+    odd = np.nonzero(a.lens > 4)[0]
+    for s in odd:                                    # the fourth own key of long sequences has a score of 0
+        a.k[int(a.table[s][0]), 3, :, 3] = 0.0
+    got, lse = a()
+    _check_rows(a, got, lse, [(s, t) for s in (0, 1, len(lens) - 1) for t in {0, tq - 1}])
+    assert np.isfinite(got).all()
