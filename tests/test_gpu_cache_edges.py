@@ -322,3 +322,35 @@ def test_attention_of_large_scores(kind, hq, hkv, hd, prefix, lens, tq, size, cu
     got, lse = a()
     _check_rows(a, got, lse, [(s, t) for s in (0, 1, len(lens) - 1) for t in {0, tq - 1}])
     assert np.isfinite(got).all()
+
+
+# ---- attention: layouts and kernels side by side ------------------------------------------
+
+
+@pytest.mark.parametrize("hq,hkv,hd,page,prefix,lens,tq,heads_first,pad", [
+    (8, 2, 128, 16, 3000, [100] * 40, 1, True, 8),      # tcgen05: 160 rows, head-major pages
+    (4, 4, 64, 24, 1500, [30] * 70, 1, True, 24),       # 70 rows, key tiles dealt out
+    (4, 1, 64, 32, 300, [200, 131], 40, True, 8),       # own keys on tcgen05 too
+    (4, 1, 32, 128, 300, [200, 131], 40, False, 40),
+    (8, 8, 128, 16, 500, [40] * 30, 1, True, 8),        # 4 warps of mma, 128 values a head
+    (3, 3, 128, 10, 400, [40] * 50, 1, True, 8),        # pages of 10
+    (1, 1, 64, 16, 500, [13000], 40, False, 0),         # 4-warp prefix, tcgen05 own keys beside it
+    (1, 1, 128, 16, 13000, [500], 24, True, 8),         # tcgen05 prefix, 4-warp own keys beside it
+])
+def test_attention_layouts_by_kernel(hq, hkv, hd, page, prefix, lens, tq, heads_first, pad, cuda):
+    import torch
+
+    a = _Attend("bf16", hq, hkv, hd, page, prefix, lens, tq, cuda, heads_first=heads_first, pad=pad)
+    got, lse = a()
+    b = len(lens)
+    q, k, v = _f64(a.q), *(_f64(x).swapaxes(1, 2) if heads_first else _f64(x) for x in (a.k, a.v))
+    for s, t in {(s, t) for s in (0, b // 2, b - 1) for t in (0, tq // 2, tq - 1)}:
+        r = s * tq + t
+        one = _attend64(q[r:r + 1, :hq * hd], k, v, a.prefix_table, prefix, a.table[s:s + 1], [lens[s] - tq + t + 1], 1,
+                        a.scale, page)
+        _check_attention("bf16", got[r:r + 1], lse[r:r + 1], one, hd)
+    assert (a.out[:, hq * hd:] == 9).all()
+    first = a.out.clone()
+    for _ in range(5):
+        a()
+        assert torch.equal(a.out, first)
