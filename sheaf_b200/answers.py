@@ -137,4 +137,5 @@ class Answers:
                                        dict(seq=seq, pos=self._ints(np.full(n, T + step)), pages=pages, base=T),
                                        dict(lens=self._ints(np.full(n, step + 1)), pages=pages, prefix_pages=prompt_pages,
                                             prefix_len=T))
+        self.s.check_device()
         return tokens, logp

@@ -237,6 +237,14 @@ class Session:
                 self._want(what, b.elem == elem and b.nbytes >= count * ELEM_SIZE[elem],
                            f"{name} has to hold {count} values of type {elem:#x}")
 
+    def check_device(self) -> None:
+        """Waits for the device and raises for what kernels have reported since the last such call: an index outside
+        its table or cache, or a wait that ran out."""
+        what = lib().sb_op_device_error()
+        if what:
+            raise SheafB200Error(3, {1: "a wait inside a kernel ran out", 2: "an index lay outside its table or cache"}
+                                 .get(what, f"device error {what}"))
+
     def kv_cache(self, n_pages: int, page_rows: int, n_heads: int, head_dim: int, elem: int = ELEM_BF16) -> "KvPages":
         """One layer's paged keys and values, [n_pages, page_rows, n_heads, head_dim] each."""
         return KvPages(self, n_pages, page_rows, n_heads, head_dim, elem)
