@@ -110,6 +110,8 @@ class Answers:
         T = len(prompt)
         if T < 1 or n < 1 or n_new < 1 or T + n_new - 1 > self.block:
             raise ValueError("prompt and answer have to fit the window")
+        if k < 1:
+            raise ValueError("a token has to be drawn from one alternative or more")
         k = min(k, self.v, 32)
         shared, own = -(-T // self.page), -(-n_new // self.page)
         self.caches = [self.s.kv_cache(shared + n * own, self.page, self.n_head, self.d // self.n_head, self.elem)

@@ -1,5 +1,5 @@
 """What kernels report about indices outside their tables reaches the callers
-of Session and Answers."""
+of Session and Answers, and what Answers refuses before it runs."""
 import numpy as np
 import pytest
 
@@ -37,3 +37,12 @@ def test_answers_ask(cuda):
         a.draw([1, 2, 3], 2, 3)
     a.s.kv_append = append
     a.draw([1, 2, 3], 2, 3)
+
+
+def test_answers_refuses_to_draw_from_nothing(cuda):
+    from tests.test_gpu_answers import _answers
+
+    _, _, a = _answers("f32")
+    for k in (0, -1):
+        with pytest.raises(ValueError):
+            a.draw([1, 2, 3], 2, 3, k=k)
