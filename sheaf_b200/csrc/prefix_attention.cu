@@ -523,7 +523,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const auto rows_of = [](Kernel k, long rows) {
     if (k == kTc) return rows > 128 ? 256 : 128;
     if (k == kSimt) return rows <= 16 ? kRows : kWideRows;
-    return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+    return k == kWarp ? 16 : (rows <= 32 ? 32 : 64);
   };
   const auto keys_of = [](Kernel k) { return k == kTc ? 128 : (k == kMma ? 64 : (k == kWarp ? 16 : kKeys)); };
   const long own_capacity = static_cast<long>(d.max_pages) * d.cache.page_rows;

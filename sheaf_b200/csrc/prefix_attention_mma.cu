@@ -8,11 +8,10 @@
 // the latency of a warp's own instructions against 8 warps an SM); more rows
 // that the tcgen05 kernel does not take:
 //
-// A block of 4 warps takes 16, 32 or 64 rows against tiles of 64 keys: with
-// 16 rows each warp takes 16 of a tile's keys, with 32 rows two warps share
-// the keys of 16 rows, with 64 rows a warp has all keys of its 16. Warps that
-// share rows keep their own maxima, sums and outputs and are joined once at
-// the end through shared memory.
+// A block of 4 warps takes 32 or 64 rows against tiles of 64 keys: with 32 rows
+// two warps share the keys of 16 rows, with 64 rows a warp has all keys of its
+// 16. Warps that share rows keep their own maxima, sums and outputs and are
+// joined once at the end through shared memory.
 //
 // Per 16 keys: s = q k^T in float32; the reference r of a row's exponents
 // 2^(s - r) rises only when some score passes it by 8, so the output is
@@ -326,7 +325,7 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, int tile_rows, M
   __syncthreads();  // the ring is free
 
   // join the warps that share rows, in the order of their keys
-  const int wk = 4 / wm;
+  const int wk = 4 / wm;  // 1 or 2
   constexpr int P = HD + 4;  // padded row of outputs
   float* buf = reinterpret_cast<float*>(&sh.kv[0][0][0]);  // [kgroup][tile_rows][P]: 64 rows at most
   float2* stat = reinterpret_cast<float2*>(buf + 64 * P);  // [kgroup][tile_rows]
@@ -402,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, HD == 128 ? 2 : 3) attn_mma_kernel(P
 
 // ---- one warp a piece: at most 16 rows -------------------------------------
 // A block is one warp with a ring of its own, 16 keys a stage, so blocks never
-// wait for one another and as many as registers and shared memory hold (9 with
+// wait for one another and as many as registers and shared memory hold (8 with
 // 128 values a head) keep the SM's copies in flight. A block takes a run of the
 // prefix or one own piece. (As many blocks as are resident, each taking every
 // so-manyth own piece, left SMs idle a quarter of the time: 512 sequences of up
