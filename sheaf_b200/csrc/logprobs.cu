@@ -199,7 +199,8 @@ struct alignas(16) RowShared {
   int count, threads;
 };
 
-// W warps per row part; rows of a block: 8 with W = 1, else 1. In a cluster
+// W warps a row (1, 4 or 8) or a part of one (16, CLUSTER); rows of a block: 8
+// with W = 1, else 1. In a cluster
 // of C blocks each takes 1 / C of the row and rank 0 joins the parts.
 template <typename T, int W, bool CLUSTER>
 __global__ void __launch_bounds__(W == 1 ? 256 : W * 32, W == 1 ? 6 : 40 / W) logprobs_kernel(FwdArgs a) {
@@ -647,26 +648,27 @@ __global__ void __launch_bounds__(256) logprobs_bwd_kernel(BwdArgs a) {
   }
 }
 
+// A warp, 4 or 8 a row.
 template <typename T, int W>
-int launch_fwd(const FwdArgs& a, int cluster, cudaStream_t s) {
+int launch_rows(const FwdArgs& a, cudaStream_t s) {
+  const int blocks = W == 1 ? (a.rows - 1) / 8 + 1 : a.rows;
+  logprobs_kernel<T, W, false><<<blocks, W == 1 ? 256 : W * 32, 0, s>>>(a);
+  return cudaPeekAtLastError() == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
+}
+// A row cut over a cluster of blocks of 16 warps.
+template <typename T>
+int launch_cut(const FwdArgs& a, int cluster, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(W == 1 ? 256 : W * 32);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * cluster);
+  cfg.blockDim = dim3(512);
   cfg.stream = s;
-  cudaError_t e;
-  if (cluster > 1) {
-    cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * cluster);
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W == 1 ? 16 : W, true>, a);
-  } else {
-    cfg.gridDim = dim3(W == 1 ? (a.rows + 7) / 8 : a.rows);
-    e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W, false>, a);
-  }
-  return e == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, 16, true>, a) == cudaSuccess ? 0 : SB_OPERR_LAUNCH;
 }
 
 template <typename T>
@@ -677,12 +679,12 @@ int fwd_t(const FwdArgs& a, cudaStream_t s) {
   // that cannot fill the SMs are cut over a cluster, up to 8 blocks of at least
   // 512 vectors a row.
   const int nvec = a.v / Elem<T>::N;
-  if (nvec <= 512) return launch_fwd<T, 1>(a, 1, s);
+  if (nvec <= 512) return launch_rows<T, 1>(a, s);
   int cluster = 1;
   while (cluster < 8 && static_cast<long>(a.rows) * cluster * 2 <= 2L * num_sms_cached() && nvec / (2 * cluster) >= 512)
     cluster *= 2;
-  if (cluster > 1) return launch_fwd<T, 16>(a, cluster, s);
-  return nvec <= 4096 ? launch_fwd<T, 4>(a, 1, s) : launch_fwd<T, 8>(a, 1, s);
+  if (cluster > 1) return launch_cut<T>(a, cluster, s);
+  return nvec <= 4096 ? launch_rows<T, 4>(a, s) : launch_rows<T, 8>(a, s);
 }
 
 }  // namespace
