@@ -517,7 +517,7 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
   const auto choose = [&](long rows, long items, long keys) {
     if (d.cache.elem == SB_ELEM_F32) return kSimt;
     if (rows <= 16) return kWarp;
-    if (keys == 0 || !tiled_rows(d.cache, 128)) return kMma;  // (there may be no memory to make a tensor map of)
+    if (d.cache.n_pages == 0 || !tiled_rows(d.cache, 128)) return kMma;  // (no tensor map of no memory)
     return rows > 64 || items * (keys / 128) >= 100L ? kTc : kMma;
   };
   const auto rows_of = [](Kernel k, long rows) {
