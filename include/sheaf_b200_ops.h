@@ -237,7 +237,11 @@ SB_API int sb_op_kv_append(const sb_kv_cache* cache, const void* qkv, int64_t ld
  * [b * tq, h_q], or NULL. A query that sees no key (lens[s] < 0 marks an idle
  * slot) gets a zero row and lse = -inf; so does one all of whose scores are
  * -inf. An infinite value makes its column inf or NaN for the queries that see
- * its key, and for no others. prefix_len = 0 is plain attention
+ * its key, and for no others. Sums are f32. With a bf16 cache and 17 query rows
+ * a key head or more (tq * h_q / n_heads to a sequence's own keys, b times that
+ * to the prefix) probabilities may be rounded to bf16 for the product with v
+ * (errors of 2.3e-3 of the outputs); with fewer they keep 16 bits (1.7e-3, the
+ * outputs' own rounding). prefix_len = 0 is plain attention
  * over a paged cache, max_pages = 0 attention to the prefix alone. lens[s]
  * beyond its table counts as the table's capacity and a page outside the
  * cache as page 0; sb_op_device_error then reports 2. scale > 0. q, out and
@@ -272,7 +276,9 @@ SB_API int sb_op_token_logprobs(uint32_t elem, const void* logits, int64_t ld, i
  * dlogits [rows, v] (row stride ldd) in the logits' type; it may be the
  * logits' own memory with ldd = ld. dlogp, dentropy f32 [rows], either NULL
  * for none (targets are needed with dlogp, entropy with dentropy). A row whose
- * lse is -inf has a zero gradient. */
+ * lse is -inf has a zero gradient. p_j = exp(z_j - lse), so the rounding of lse
+ * to f32, |lse| 2^-24, is an error of log p_j: far from zero (|lse| > 10^5)
+ * take the row's maximum off the logits first. */
 SB_API int sb_op_token_logprobs_bwd(uint32_t elem, const void* logits, int64_t ld, int32_t rows, int32_t v,
                                     const void* targets, float temperature, const void* lse, const void* entropy,
                                     const void* dlogp, const void* dentropy, void* dlogits, int64_t ldd,

@@ -26,8 +26,9 @@ from .runtime import Buffer, Session, SheafB200Error
 class Answers:
     """Draws answers to a prompt from a nanoGPT model.
 
-    ``logits`` of the last step and ``scores`` stay on the device: what a
-    policy-gradient step differentiates (``Session.token_logprobs_vjp``)."""
+    ``logits`` of the last step and ``scores`` stay on the device. The gradient
+    of a policy-gradient step in them is ``Session.token_logprobs_vjp``; it ends
+    at the logits, and nothing here takes it on to the parameters."""
 
     def __init__(self, session: Session, leaves: list[Buffer], *, n_layer: int, n_head: int, n_embd: int,
                  block_size: int, vocab_size: int, page_rows: int = 16):

@@ -233,8 +233,9 @@ static bool on_values(const void* p, uint32_t elem) {
   return reinterpret_cast<uintptr_t>(p) % (elem == SB_ELEM_F32 ? 4 : 2) == 0;
 }
 
-// A usable cache description: strides that keep every 16-byte vector aligned
-// (rows of a head never overlap a neighbour's by less than head_dim).
+// A usable cache description: strides that keep every 16-byte vector aligned.
+// (Rows may overlap or coincide, as a stride of 0 has them: attention reads
+// them as they are, an append to such rows writes them in no order.)
 static int check_cache(const sb_kv_cache* c) {
   if (!c || !float_elem(c->elem)) return SB_OPERR_ARGS;
   if (c->n_heads <= 0 || c->page_rows <= 0 || c->n_pages < 0) return SB_OPERR_ARGS;

@@ -12,8 +12,8 @@
 // further on), for HPT heads, so that the angles are read once for HPT
 // heads and 2 HPT loads are in flight. Moving the bytes bounds it: 16384 tokens
 // of 32 + 8 + 8 heads of 128 in bf16, 403 MB, take 62 us at the measured copy
-// rate; 70 without rotation, 79 with pairs, 83 with halves (two heads a thread,
-// four blocks an SM; one head 101, four heads 99); float32 124, 0.99 of the
+// rate; 69 without rotation, 78 with pairs, 83 with halves (two heads a thread,
+// four blocks an SM; one head 101, four heads 99); float32 126, 0.97 of the
 // rate. The angles' 64 bytes a thread, from L1, are what bf16 pays for.
 #include <cuda_bf16.h>
 

@@ -21,10 +21,11 @@
 // logits that reach it become candidates: about 64 ln(64 / (64 - k)) of them.
 //
 // Reading the logits bounds it: 8192 x 50304 bf16, 824 MB, take 126 us at the
-// measured copy rate, and 152 us without alternatives, 184 with 8 (0.68). What
-// is left: the exponentials alone take 0.57 of the time on their unit, and a
-// block does not read while it joins a row's statistics and looks up the
-// alternatives. The VJP reads and writes once: 4096 x 50304 in 147 us, 0.86.
+// measured copy rate, and 164-170 us without alternatives, 185 with 8 where calls
+// follow one another, 195 (0.64) each with new logits. What is left: the
+// exponentials alone take 0.57 of the time on their unit, and a block does not
+// read while it joins a row's statistics and looks up the alternatives. The VJP
+// reads and writes once: 4096 x 50304 in 147 us (0.86) and 152 likewise.
 #include <cuda_bf16.h>
 
 #include <algorithm>

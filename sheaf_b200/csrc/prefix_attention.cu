@@ -188,7 +188,7 @@ __device__ void attend_piece(const PaArgs& a, const PaPiece& w, SimtShared<HD>& 
 // keys, then 4 rows of HD / 8 output columns, so that each 16 bytes read from
 // shared memory serve 8 or more multiply-adds and these bound the kernel.
 // (With 4 rows a warp the shared-memory reads do: 8 x 41 queries of 4 heads of
-// 128 behind 10565 keys took 590 us; this takes 308, 23 TFLOP/s, with 8 warps
+// 128 behind 10565 keys took 590 us; this takes 293, 24 TFLOP/s, with 8 warps
 // an SM, too few to cover the latency of the arithmetic.)
 constexpr int kWideRows = 64;
 
@@ -555,9 +555,12 @@ bool plan_of(const PrefixAttnDesc& d, Plan& p) {
     // and the own keys' blocks fill the others and, as they come free, these.
     // A 256-row tile costs an SM as much as 7 of the warps' 16-key tiles; about
     // a third of the own capacity is counted, since lengths are on the device
-    // and too many SMs cost less than too few. (64 x 32 queries behind 8192
-    // shared and up to 512 own keys 49 -> 41 us, counting a sixth 48; 100 of
-    // them behind 20000, 96 -> 73.) Beyond 24 tiles, or an eighth more than all
+    // and too many SMs cost less than too few. That suits lengths spread over
+    // the capacity (64 x 32 queries behind 8192 and 0..512 own keys 39 us, in a
+    // row of calls) as well as equal ones below it (256 each: 40, 8 each: 38);
+    // with the capacity full the own keys end last (512 each: 51). Against one
+    // block an SM, other work between the calls: 49 -> 41 us, counting a sixth
+    // 48; 100 of them behind 20000, 96 -> 73. Beyond 24 tiles, or an eighth more than all
     // SMs would give, nothing is gained (512 behind 16384 and up to 256: 201 at
     // half as many again, 198 here), and the prefix could end last (512 behind
     // 400 and up to 600: 136 us, 282 without this limit).

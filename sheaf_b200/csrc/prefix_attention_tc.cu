@@ -14,7 +14,11 @@
 // A block takes up to 256 rows, two tiles of 128, against tiles of 128 keys;
 // 12 warps:
 //   warps 0-3, 4-7  softmax of row tile 0, 1: thread = row; P goes back to TMEM as bf16 over the
-//             columns of S it came from, the A operand of P V. The reference
+//             columns of S it came from, the A operand of P V. (One bf16, with an
+//             error of the outputs against 64 bits of 2.3e-3 where the sum of two
+//             gives the outputs' own rounding, 1.7e-3: a second term would double
+//             the products with V in a kernel that products bound. From 17 rows on
+//             this holds where reading bounds it, too.) The reference
 //             r of a row's exponents 2^(s - r) rises only when their sum over a
 //             tile passes 2^15, so O (in TMEM) is rescaled rarely.
 //   warp 8    TMEM owner, one thread issues the UMMAs: for row tile x
