@@ -354,3 +354,133 @@ def test_attention_layouts_by_kernel(hq, hkv, hd, page, prefix, lens, tq, heads_
     for _ in range(5):
         a()
         assert torch.equal(a.out, first)
+
+
+# ---- offsets beyond 32 bits, and graphs -----------------------------------------------------
+
+
+def _far_pages(kind, rows, heads, hd, dev):
+    """Nine pages 2^28 elements apart, the last one beyond 2^31, as views of one allocation."""
+    import torch
+
+    flat = torch.empty(2 ** 31 + 2 ** 18, device=dev, dtype=torch.float32 if kind == "f32" else torch.bfloat16)
+    return flat.as_strided((9, rows, heads, hd), (2 ** 28, heads * hd, hd, 1))
+
+
+@pytest.mark.parametrize("kind,hq,hkv,hd,prefix,lens,tq", [
+    ("bf16", 4, 2, 64, 20, [9, 14], 1),              # a warp
+    ("bf16", 8, 1, 128, 30, [9, 14, 16], 3),         # 4 warps
+    ("bf16", 8, 1, 128, 64, [40, 64], 40),           # tcgen05
+    ("f32", 4, 2, 64, 20, [9, 14], 1),
+    ("f32", 8, 1, 128, 30, [9, 14, 16], 3),
+])
+def test_attention_over_pages_beyond_32_bits(kind, hq, hkv, hd, prefix, lens, tq, cuda):
+    a = _Attend(kind, hq, hkv, hd, 64, prefix, lens, tq, cuda)
+    want, want_lse = a()
+    far = []
+    for x in (a.k, a.v):
+        y = _far_pages(kind, 64, hkv, hd, cuda)
+        y[9 - x.shape[0]:].copy_(x)
+        far.append(y)
+    shift = 9 - a.k.shape[0]
+    a.k, a.v = far
+    a.prefix_table, a.table = a.prefix_table + shift, a.table + shift
+    got, lse = a()
+    assert np.array_equal(got, want) and np.array_equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_append_beyond_32_bits(kind, cuda):
+    import torch
+    import sheaf_b200 as sb
+
+    hq, hkv, hd, n, page = 2, 2, 64, 70, 32
+    width = (hq + 2 * hkv) * hd
+    qkv = torch.randn(n, width, device=cuda).to(torch.float32 if kind == "f32" else torch.bfloat16)
+    k, v = (_far_pages(kind, page, hkv, hd, cuda) for _ in range(2))
+    pages = [8, 0, 7]
+    for x in (k, v):
+        x[pages] = 0
+    q = torch.zeros(n, hq * hd, device=cuda, dtype=qkv.dtype)
+    seq, pos, table = _i(np.zeros(n), cuda), _i(np.arange(n), cuda), _i([pages], cuda)
+    assert sb.lib().sb_op_kv_append(_cache((k, v)), qkv.data_ptr(), width, n, hq, q.data_ptr(), hq * hd, seq.data_ptr(),
+                                    pos.data_ptr(), 0, table.data_ptr(), 1, 3, 0, 0, None, None, 0, _stream()) == 0
+    x = qkv.view(n, hq + 2 * hkv, hd)
+    assert torch.equal(q, x[:, :hq].reshape(n, -1))
+    for c, part in ((k, x[:, hq:hq + hkv]), (v, x[:, hq + hkv:])):
+        assert torch.equal(c[pages].reshape(-1, hkv, hd)[:n], part)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("v", [1000, 9000])
+def test_logprobs_of_rows_beyond_32_bits(kind, v, cuda):
+    import torch
+    import sheaf_b200 as sb
+
+    L, ld, rows, k = sb.lib(), 2 ** 30 + 8, 3, 4
+    flat = torch.empty(2 * ld + v, device=cuda, dtype=torch.float32 if kind == "f32" else torch.bfloat16)
+    x = flat.as_strided((rows, v), (ld, 1))
+    near = torch.randn(rows, v, device=cuda).to(flat.dtype)
+    x.copy_(near)
+    t, g = _t([5, 0, v - 1], "f32", cuda), _t([1.0, -2.0, 0.5], "f32", cuda)
+
+    def score(p, ld):
+        o = torch.zeros(3, rows, device=cuda)
+        ids = torch.zeros(rows, k, device=cuda, dtype=torch.int32)
+        alt = torch.zeros(rows, k, device=cuda)
+        assert L.sb_op_token_logprobs(ELEM[kind], p.data_ptr(), ld, rows, v, t.data_ptr(), 1.0, o[0].data_ptr(),
+                                      o[1].data_ptr(), o[2].data_ptr(), k, ids.data_ptr(), alt.data_ptr(),
+                                      _stream()) == 0
+        return o, ids, alt
+
+    def grad(p, ld, o):
+        assert L.sb_op_token_logprobs_bwd(ELEM[kind], p.data_ptr(), ld, rows, v, t.data_ptr(), 1.0, o[2].data_ptr(),
+                                          o[1].data_ptr(), g.data_ptr(), g.data_ptr(), p.data_ptr(), ld, _stream()) == 0
+
+    want, got = score(near, v), score(flat, ld)
+    assert torch.equal(want[1], got[1])
+    assert (want[0] - got[0]).abs().max() < 1e-5 and (want[2] - got[2]).abs().max() < 1e-5
+    grad(near, v, want[0])
+    grad(flat, ld, want[0])
+    assert torch.equal(near, x)
+
+
+@pytest.mark.parametrize("kind,hq,hkv,hd,prefix,lens,tq", [
+    ("bf16", 4, 4, 64, 2000, [40] * 80, 1),     # tcgen05, and a warp's blocks beside it
+    ("bf16", 2, 2, 64, 300, [20] * 12, 3),      # 4 warps, and a warp's blocks beside them
+    ("bf16", 2, 1, 64, 0, [300, 5], 40),
+    ("f32", 4, 2, 64, 300, [5, 60], 2),
+])
+def test_attention_in_a_graph(kind, hq, hkv, hd, prefix, lens, tq, cuda):
+    """Captured once after a first call, replayed with other queries and lengths in the same places."""
+    import torch
+    import sheaf_b200 as sb
+
+    a = _Attend(kind, hq, hkv, hd, 16, prefix, lens, tq, cuda)
+    L, c, b = sb.lib(), _cache((a.k, a.v)), len(lens)
+    size = L.sb_op_prefix_attention_workspace_size(c, b, tq, hq, prefix, a.table.shape[1])
+    ws = torch.full((size // 4 + 4,), float("nan"), device=cuda)
+    pt, t, ln = _i(a.prefix_table, cuda), _i(a.table, cuda), _i(a.lens, cuda)
+    q, out = a.q.clone(), torch.zeros_like(a.out)
+
+    def attend():
+        assert L.sb_op_prefix_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), None, b, tq, hq,
+                                        a.scale, pt.data_ptr(), prefix, t.data_ptr(), a.table.shape[1], ln.data_ptr(),
+                                        ws.data_ptr(), size, _stream()) == 0
+
+    attend()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            attend()
+    for i in range(4):
+        a.lens = np.maximum(np.array(lens) - i, 0)
+        a.q.mul_(0.75)
+        want, _ = a()
+        q.copy_(a.q)
+        ln.copy_(_i(a.lens, cuda))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(_f64(out).reshape(want.shape), want)
